@@ -151,6 +151,12 @@ struct g4a_ctx {
     hipFunction_t slice_cols = nullptr;
     hipFunction_t rms_rows = nullptr;        // (residual +) RMSNorm (* scalar) over rows of any width
     hipFunction_t embed_f32 = nullptr;
+    // the paged KV cache: [head_dim 64, 128, 256, 512][f32, bf16 pages]
+    hipFunction_t page_map[2] = {};  // [256, 1024 threads]
+    hipFunction_t paged_producer[4][2] = {};
+    hipFunction_t paged_decode[4][2] = {};
+    hipFunction_t paged_gather[2] = {};
+    uint32_t* ticket = nullptr;  // g4a_page_map's: 0 between launches
     // RoPE frequency tables theta^(-2j/rot), one per (theta, rotary_dim) seen
     struct FreqTable {
         float theta;
@@ -899,6 +905,25 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
         if (int rc = get_fn(ctx, &ctx->rms_rows, "g4a_rms_rows")) return bail(rc);
         if (int rc = get_fn(ctx, &ctx->embed_f32, "g4a_embed_rows_f32")) return bail(rc);
     }
+    if (int rc = get_fn(ctx, &ctx->page_map[0], "g4a_page_map_t256")) return bail(rc);
+    if (int rc = get_fn(ctx, &ctx->page_map[1], "g4a_page_map_t1024")) return bail(rc);
+    for (int t = 0; t < 2; ++t) {
+        const char* const type = t ? "bf16" : "f32";
+        char name[64];
+        for (int d = 0; d < 4; ++d) {
+            snprintf(name, sizeof name, "g4a_paged_producer_d%d_%s", 64 << d, type);
+            if (int rc = get_fn(ctx, &ctx->paged_producer[d][t], name)) return bail(rc);
+            snprintf(name, sizeof name, "g4a_paged_decode_d%d_%s", 64 << d, type);
+            if (int rc = get_fn(ctx, &ctx->paged_decode[d][t], name)) return bail(rc);
+        }
+        snprintf(name, sizeof name, "g4a_paged_gather_%s", type);
+        if (int rc = get_fn(ctx, &ctx->paged_gather[t], name)) return bail(rc);
+    }
+    if (hipMalloc(reinterpret_cast<void**>(&ctx->ticket), 256) != hipSuccess ||
+        hipMemset(ctx->ticket, 0, 256) != hipSuccess) {
+        fail(ctx, G4A_E_NOMEM, "ticket allocation failed");
+        return bail(G4A_E_NOMEM);
+    }
     if (hipMalloc(reinterpret_cast<void**>(&ctx->dummy), 4096) != hipSuccess ||
         hipMemset(ctx->dummy, 0, 4096) != hipSuccess) {
         fail(ctx, G4A_E_NOMEM, "dummy buffer allocation failed");
@@ -928,6 +953,7 @@ void g4a_destroy(g4a_ctx* ctx) {
         ctx->book->ctx = nullptr;
     }
     if (ctx->dummy) hipFree(ctx->dummy);
+    if (ctx->ticket) hipFree(ctx->ticket);
     if (ctx->pos_dev) hipFree(ctx->pos_dev);
     for (auto& ft : ctx->freq_tables) hipFree(ft.dev);
     for (auto& st : ctx->sc_tables) hipFree(st.dev);
@@ -2284,6 +2310,166 @@ int g4a_attn_producer_devpos(g4a_ctx* ctx, const g4a_producer_args* a, const uin
     if (a->T != 1) return fail(ctx, G4A_E_UNSUPPORTED, "a device-position producer step has one token (T = %u)", a->T);
     if (a->positions) return fail(ctx, G4A_E_ARG, "a device-position producer step takes its position from `pos`");
     return producer_run(ctx, a, pos, max_pos);
+}
+
+// ---- paged KV cache ----------------------------------------------------------
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Index of a paged cache's head_dim among the kernels'.
+int paged_dh(uint32_t Dh) { return Dh == 64 ? 0 : Dh == 128 ? 1 : Dh == 256 ? 2 : 3; }
+
+// Checks a paged cache's tables (`tables`) and pools and widths (`pools`), and gives
+// the kernels' form of it.
+int paged_cache(g4a_ctx* ctx, const g4a_paged_cache* c, bool tables, bool pools, G4aPaged* out) {
+    if (!c) return fail(ctx, G4A_E_ARG, "null cache");
+    if (c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)))
+        return fail(ctx, G4A_E_UNSUPPORTED, "page_size %u is not a power of two from 16 to 65536", c->page_size);
+    if (c->n_pages == 0 || uint64_t(c->n_pages) * c->page_size >= G4A_NO_ROW)
+        return fail(ctx, G4A_E_SHAPE, "%u pages of %u tokens: slots must be 0 .. 2^32 - 2", c->n_pages, c->page_size);
+    if (c->ring > 1) return fail(ctx, G4A_E_ARG, "ring %u is neither 0 nor 1", c->ring);
+    *out = G4aPaged{c->k_pages, c->v_pages, c->block_table, c->kv_len, c->page_stride, c->n_seqs, c->pages_per_seq,
+                    c->n_pages, uint32_t(__builtin_ctz(c->page_size)), c->Hkv, c->Dh, c->ring};
+    if (tables && c->n_seqs) {
+        if (!c->block_table || !c->kv_len) return fail(ctx, G4A_E_ARG, "null block_table / kv_len");
+        if (c->pages_per_seq == 0 || uint64_t(c->pages_per_seq) * c->page_size >= G4A_NO_ROW ||
+            uint64_t(c->n_seqs) * c->pages_per_seq >= G4A_NO_ROW)
+            return fail(ctx, G4A_E_SHAPE, "tables of %u x %u pages of %u tokens: a sequence's tokens and the table's "
+                        "entries must be 1 .. 2^32 - 2", c->n_seqs, c->pages_per_seq, c->page_size);
+    }
+    if (pools) {
+        if (c->Dh != 64 && c->Dh != 128 && c->Dh != 256 && c->Dh != 512)
+            return fail(ctx, G4A_E_UNSUPPORTED, "head_dim %u: paged caches have 64, 128, 256 or 512", c->Dh);
+        if (c->Hkv == 0 || c->Hkv > 1024) return fail(ctx, G4A_E_UNSUPPORTED, "Hkv %u is not 1 .. 1024", c->Hkv);
+        if (c->kv_type != G4A_KV_F32 && c->kv_type != G4A_KV_BF16)
+            return fail(ctx, G4A_E_ARG, "kv_type %u is no g4a_kv_type", c->kv_type);
+        if (!c->k_pages || !c->v_pages || !aligned16(c->k_pages) || !aligned16(c->v_pages))
+            return fail(ctx, G4A_E_ARG, "k_pages / v_pages null or not 16-byte aligned");
+        const uint64_t page = uint64_t(c->page_size) * c->Hkv * c->Dh;
+        if (c->page_stride && (c->page_stride % 8 || c->page_stride < page || c->page_stride >> 40))
+            return fail(ctx, G4A_E_SHAPE, "page_stride %llu: a multiple of 8 values from the page's %llu on, below 2^40",
+                        (unsigned long long)c->page_stride, (unsigned long long)page);
+        if (!c->page_stride) out->page_stride = page;
+    }
+    return G4A_OK;
+}
+
+}  // namespace
+
+int g4a_page_map(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_page_map_args* a) {
+    if (!ctx) return fail(ctx, G4A_E_ARG, "null ctx");
+    G4aPageMapParams p{};
+    if (int rc = paged_cache(ctx, cache, true, false, &p.c)) return rc;
+    if (!a) return fail(ctx, G4A_E_ARG, "null args");
+    if (a->rows >> 31) return fail(ctx, G4A_E_SHAPE, "%u rows: below 2^31", a->rows);
+    if (a->rows_per_seq && uint64_t(a->rows_per_seq) * cache->n_seqs != a->rows)
+        return fail(ctx, G4A_E_SHAPE, "%u rows are not %u for each of %u sequences", a->rows, a->rows_per_seq,
+                    cache->n_seqs);
+    if (cache->n_seqs == 0 && a->rows == 0) return G4A_OK;
+    if (a->rows && (!a->slots || !a->positions)) return fail(ctx, G4A_E_ARG, "null slots / positions");
+    if (!a->free_pages || !a->free_state || a->free_cap == 0)
+        return fail(ctx, G4A_E_ARG, "null free_pages / free_state or an empty free ring");
+    p.add = a->new_len;
+    p.shared = a->shared_pages;
+    p.free_pages = a->free_pages;
+    p.free_state = a->free_state;
+    p.free_cap = a->free_cap;
+    p.rows = a->rows;
+    p.rows_per_seq = a->rows_per_seq;
+    p.slots = a->slots;
+    p.positions = a->positions;
+    p.row_start = a->row_start;
+    p.added = a->added;
+    p.len_out = a->kv_len_out ? a->kv_len_out : cache->kv_len;
+    p.state_out = a->free_state_out ? a->free_state_out : a->free_state;
+    p.ticket = ctx->ticket;
+    // a workgroup takes 4 rows a thread, and all sequences' scans
+    const uint32_t threads = cache->n_seqs <= 256 ? 256 : 1024;
+    const uint32_t wgs = std::min<uint32_t>(std::max<uint32_t>(1, (a->rows + 4 * threads - 1) / (4 * threads)),
+                                            uint32_t(std::max(ctx->cu_count, 1)));
+    return launch(ctx, ctx->page_map[threads == 1024], dim3(wgs, 1, 1), dim3(threads, 1, 1), p, "page map", true);
+}
+
+int g4a_attn_producer_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_paged_producer_args* a) {
+    if (!ctx) return fail(ctx, G4A_E_ARG, "null ctx");
+    G4aPagedProducerParams p{};
+    if (int rc = paged_cache(ctx, cache, false, true, &p.c)) return rc;
+    if (!a) return fail(ctx, G4A_E_ARG, "null args");
+    const uint32_t rot = a->rotary_dim;
+    if (rot % 2 != 0 || rot > cache->Dh)
+        return fail(ctx, G4A_E_ARG, "rotary_dim %u must be even and <= head_dim %u", rot, cache->Dh);
+    if ((a->k == nullptr) != (a->v == nullptr)) return fail(ctx, G4A_E_ARG, "k and v come together");
+    if (a->Hq == 0 || a->Hq > 65536) return fail(ctx, G4A_E_UNSUPPORTED, "Hq %u is not 1 .. 65536", a->Hq);
+    p.heads = a->Hq + (a->k ? 2 * cache->Hkv : 0);
+    const uint64_t rows = uint64_t(a->T) * p.heads;
+    if (rows >> 32) return fail(ctx, G4A_E_SHAPE, "too many rows (%llu)", (unsigned long long)rows);
+    if (a->T == 0) return G4A_OK;
+    if (!a->q || !a->q_out || !a->positions || (a->k && !a->slots))
+        return fail(ctx, G4A_E_ARG, "null q / q_out / positions / slots");
+    for (const void* x : {(const void*)a->q, (const void*)a->k, (const void*)a->v, (const void*)a->q_norm,
+                          (const void*)a->k_norm, (const void*)a->q_out})
+        if (!aligned16(x)) return fail(ctx, G4A_E_ARG, "rows and norm weights must be 16-byte aligned");
+    if (rot)
+        if (int rc = freq_table(ctx, a->theta, rot, &p.freq)) return rc;
+    p.q = a->q;
+    p.kx = a->k;
+    p.vx = a->v;
+    p.q_norm = a->q_norm;
+    p.k_norm = a->k_norm;
+    p.q_out = a->q_out;
+    p.positions = a->positions;
+    p.slots = a->slots;
+    p.T = a->T;
+    p.Hq = a->Hq;
+    p.rotary_dim = rot;
+    p.eps = a->eps;
+    const uint32_t per_wg = 4 * std::max<uint32_t>(1, 256 / cache->Dh);
+    return launch(ctx, ctx->paged_producer[paged_dh(cache->Dh)][cache->kv_type],
+                  dim3(uint32_t((rows + per_wg - 1) / per_wg), 1, 1), dim3(256, 1, 1), p, "paged producer", true);
+}
+
+int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_paged_attn_args* a) {
+    if (!ctx) return fail(ctx, G4A_E_ARG, "null ctx");
+    G4aPagedAttnParams p{};
+    if (int rc = paged_cache(ctx, cache, true, true, &p.c)) return rc;
+    if (!a) return fail(ctx, G4A_E_ARG, "null args");
+    if (a->Hq == 0 || a->Hq % cache->Hkv || a->Hq > 65535)
+        return fail(ctx, G4A_E_SHAPE, "Hq %u: a multiple of Hkv %u, at most 65535", a->Hq, cache->Hkv);
+    if (!(a->attn_softcap >= 0.0f)) return fail(ctx, G4A_E_ARG, "attn_softcap %g is negative", a->attn_softcap);
+    if (cache->n_seqs == 0) return G4A_OK;
+    if (!a->q || !a->out || !aligned16(a->q) || !aligned16(a->out))
+        return fail(ctx, G4A_E_ARG, "q / out null or not 16-byte aligned");
+    p.q = a->q;
+    p.out = a->out;
+    p.Hq = a->Hq;
+    p.window = a->sliding_window;
+    p.scale = a->scale;
+    p.softcap = a->attn_softcap;
+    return launch(ctx, ctx->paged_decode[paged_dh(cache->Dh)][cache->kv_type], dim3(cache->n_seqs, a->Hq, 1),
+                  dim3(256, 1, 1), p, "paged decode", true);
+}
+
+int g4a_kv_gather_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, uint32_t seq, uint32_t pos0, uint32_t n,
+                        float* k_out, float* v_out) {
+    if (!ctx) return fail(ctx, G4A_E_ARG, "null ctx");
+    G4aPagedGatherParams p{};
+    if (int rc = paged_cache(ctx, cache, true, true, &p.c)) return rc;
+    if (seq >= cache->n_seqs) return fail(ctx, G4A_E_ARG, "sequence %u of %u", seq, cache->n_seqs);
+    if (uint64_t(pos0) + n >= G4A_NO_ROW) return fail(ctx, G4A_E_SHAPE, "positions %u + %u pass 2^32 - 2", pos0, n);
+    if (n == 0) return G4A_OK;
+    if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
+        return fail(ctx, G4A_E_ARG, "k_out / v_out null or not 16-byte aligned");
+    p.k_out = k_out;
+    p.v_out = v_out;
+    p.seq = seq;
+    p.pos0 = pos0;
+    p.n = n;
+    // about 16 KiB of rows a workgroup
+    while (p.rows_shift < p.c.page_shift && (uint64_t(cache->Hkv) * cache->Dh * 4 << p.rows_shift) < 16384) ++p.rows_shift;
+    const uint32_t groups = ((pos0 + n - 1) >> p.rows_shift) - (pos0 >> p.rows_shift) + 1;
+    return launch(ctx, ctx->paged_gather[cache->kv_type], dim3(groups, 2, 1), dim3(256, 1, 1), p, "paged gather", true);
 }
 
 struct g4a_graph {

@@ -7,3 +7,5 @@
 #include "linear_q.hip"
 #include "linear_mm.hip"
 #include "elementwise.hip"
+#include "paged.hip"
+#include "attn_paged.hip"

@@ -340,3 +340,72 @@ struct G4aEmbedF32Params {
     uint32_t T, D;
     float scale;
 };
+
+// ---- paged KV cache (paged.hip, attn_paged.hip) ----
+// Token t of sequence b sits on page table[b * per_seq + e], e = t >> page_shift (a
+// ring: modulo per_seq), at row t & (page size - 1) of it; a row is Hkv * Dh values.
+// An entry of n_pages or more names no page.
+struct G4aPaged {
+    void* k;                // [n_pages] pages, page_stride values apart, f32 or bf16
+    void* v;
+    uint32_t* table;        // device [n_seqs][per_seq]
+    const uint32_t* len;    // device [n_seqs]: tokens in the cache
+    uint64_t page_stride;
+    uint32_t n_seqs, per_seq, n_pages, page_shift, Hkv, Dh;
+    uint32_t ring;
+};
+
+constexpr uint32_t G4A_NO_ROW32 = 0xFFFFFFFFu;  // G4A_NO_ROW, G4A_SEQ_END
+
+// One step's pages, slots and positions (g4a_page_map). The outputs may be the inputs'
+// buffers: with more than one workgroup the last to finish its reads (ticket) writes them.
+struct G4aPageMapParams {
+    G4aPaged c;
+    const uint32_t* add;     // device [n_seqs] new tokens, G4A_SEQ_END: the sequence ends; null: one each
+    const uint32_t* shared;  // device [n_seqs] leading pages that stay when the sequence ends, or null
+    uint32_t* free_pages;    // device [free_cap], a ring
+    const uint32_t* free_state;  // device {first, count}
+    uint32_t free_cap;
+    uint32_t rows, rows_per_seq;  // rows_per_seq 0: packed rows
+    uint32_t* slots;         // device [rows]
+    uint32_t* positions;     // device [rows]
+    uint32_t* row_start;     // device [n_seqs + 1] or null
+    uint32_t* added;         // device [n_seqs] or null
+    uint32_t* len_out;
+    uint32_t* state_out;
+    uint32_t* ticket;        // device counter, 0 between launches
+};
+
+// Norm, RoPE and paged write of T tokens' q, k and v rows (g4a_paged_producer_*).
+struct G4aPagedProducerParams {
+    G4aPaged c;
+    const float* q;          // [T, Hq, Dh]
+    const float* kx;         // [T, Hkv, Dh] or null
+    const float* vx;
+    const float* q_norm;     // [Dh] or null: not normalised
+    const float* k_norm;
+    float* q_out;
+    const uint32_t* positions;  // device [T]; G4A_NO_ROW: the token's rows are left alone
+    const uint32_t* slots;      // device [T]; G4A_NO_ROW: no K/V write
+    const float* freq;          // [rotary_dim / 2]
+    uint32_t T, Hq, heads, rotary_dim;  // heads: rows of a token (Hq, or Hq + 2 Hkv)
+    float eps;
+};
+
+// Tokens [pos0, pos0 + n) of sequence seq in order, as f32 (g4a_paged_gather_*).
+struct G4aPagedGatherParams {
+    G4aPaged c;
+    float* k_out;            // [n, Hkv, Dh]
+    float* v_out;
+    uint32_t seq, pos0, n;
+    uint32_t rows_shift;     // log2 of the tokens of a workgroup (within one page)
+};
+
+// One query of every sequence over its pages (g4a_paged_decode_*).
+struct G4aPagedAttnParams {
+    G4aPaged c;
+    const float* q;          // [n_seqs, Hq, Dh]
+    float* out;              // [n_seqs, Hq * Dh]
+    uint32_t Hq, window;
+    float scale, softcap;
+};

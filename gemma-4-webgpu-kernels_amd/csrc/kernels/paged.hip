@@ -1,0 +1,338 @@
+// The paged KV cache's bookkeeping for gfx950: the page map of a step, the
+// attention producer that writes into pages, and the copy of cached tokens in
+// order. The reference has no paged cache (its KVCache grows one buffer per
+// layer, rust/src/kvcache.rs:49-62). Layout: G4aPaged (g4a_params.h).
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "g4a_math.h"
+#include "g4a_params.h"
+
+namespace {
+
+// Inclusive sums over a workgroup of T threads of two values; `tot` gets the
+// workgroup's sums. Waves first (shuffles), then the wave sums through LDS.
+template <int T, typename A, typename B>
+__device__ __forceinline__ void block_scan(A& a, B& b, A& tot_a, B& tot_b) {
+    __shared__ A wa[T / 64];
+    __shared__ B wb[T / 64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const A ua = __shfl_up(a, d);
+        const B ub = __shfl_up(b, d);
+        if (lane >= d) {
+            a += ua;
+            b += ub;
+        }
+    }
+    __syncthreads();  // the sums of an earlier call have been read
+    if (lane == 63) {
+        wa[w] = a;
+        wb[w] = b;
+    }
+    __syncthreads();
+    A ba = 0;
+    B bb = 0;
+    tot_a = 0;
+    tot_b = 0;
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) {
+        if (i < w) {
+            ba += wa[i];
+            bb += wb[i];
+        }
+        tot_a += wa[i];
+        tot_b += wb[i];
+    }
+    a += ba;
+    b += bb;
+}
+
+// Last i in [0, n) with start[i] <= x (start ascending, start[0] <= x).
+__device__ __forceinline__ uint32_t last_at_or_before(const uint32_t* start, uint32_t n, uint32_t x) {
+    uint32_t lo = 0;
+    for (uint32_t step = 1024; step > 0; step >>= 1)
+        if (lo + step < n && start[lo + step] <= x) lo += step;
+    return lo;
+}
+
+// A step's page map. With had = ceil(len / page size), capped at the table's entries,
+// and need = ceil((len + add) / page size) - had, likewise capped, a sequence takes
+// pages first + C - need .. first + C - 1 of the free ring, C the running sum of need:
+// it goes on if C <= count or need = 0, if its tokens fit its table and its rows, and,
+// packed, if the running sum of rows fits. Token i of it is row start + i at position
+// len + i; the row of a page's first token also writes the table entry. Sequences that
+// end put their pages at the ring's end.
+//
+// Every workgroup runs the scans over all sequences, T of them at a time, and writes
+// its share of each chunk's rows: the scans are a microsecond of latency, less than a
+// second launch. Lengths and ring state are written by workgroup 0 where they have
+// buffers of their own, else by the workgroup that draws the last ticket, which is
+// after every other's reads of them.
+template <int T>
+__device__ __forceinline__ void page_map(const G4aPageMapParams& p) {
+    __shared__ uint32_t s_start[T], s_len[T], s_had[T], s_base[T], s_added[T], s_rel[T], s_keep[T];
+    __shared__ uint32_t s_last;
+    const G4aPaged& c = p.c;
+    const uint32_t tid = threadIdx.x, shift = c.page_shift, low = (1u << shift) - 1, P = c.per_seq;
+    const uint32_t first = p.free_state[0] % p.free_cap, count = min(p.free_state[1], p.free_cap);
+    const uint64_t room = (uint64_t)P << shift;
+    const bool apart = p.len_out != c.len && p.state_out != p.free_state;
+    auto pages = [&](uint64_t tokens) { return (uint32_t)min((tokens + low) >> shift, (uint64_t)P); };
+    auto ring_page = [&](uint32_t i) { return p.free_pages[(uint32_t)(((uint64_t)first + i) % p.free_cap)]; };
+
+    // One pass over all sequences; `rows`: write this workgroup's rows and released
+    // pages, `commit`: write the per-sequence outputs and the ring's state.
+    auto pass = [&](bool rows, bool commit) {
+        uint64_t row0 = 0;                // rows of the chunks before
+        uint32_t need0 = 0, rel0 = 0;     // pages demanded, pages released
+        uint32_t taken = 0;               // pages taken
+        for (uint32_t b0 = 0; b0 < c.n_seqs; b0 += T) {
+            const uint32_t b = b0 + tid;
+            const bool is = b < c.n_seqs;
+            const uint32_t len = is ? c.len[b] : 0u;
+            const uint32_t add = is ? (p.add ? p.add[b] : 1u) : 0u;
+            const bool ends = is && add == G4A_NO_ROW32;
+            const uint32_t want = ends ? 0u : add;
+            const uint64_t after = (uint64_t)len + want;
+            const bool fits = (c.ring ? after < G4A_NO_ROW32 : after <= room) &&
+                              (p.rows_per_seq == 0 || want <= p.rows_per_seq);
+            const uint32_t had = pages(len);
+            const uint32_t need = fits && want ? pages(after) - had : 0u;
+            const uint32_t keep = ends && p.shared ? min(p.shared[b], had) : 0u;
+            uint32_t cn = need, cr = ends ? had - keep : 0u, tn, tr;
+            const uint32_t rel = cr;
+            block_scan<T>(cn, cr, tn, tr);
+            cn += need0;
+            const bool goes = fits && (need == 0 || cn <= count);
+            uint64_t rn = goes ? want : 0u, trows;
+            uint32_t ta = 0, tt;
+            const uint32_t mine = (uint32_t)rn;
+            block_scan<T>(rn, ta, trows, tt);
+            rn += row0;  // rows up to and with this sequence's
+            const bool in = goes && (p.rows_per_seq != 0 || rn <= p.rows);
+            const uint32_t added = in ? mine : 0u;
+            // (of sequences that go but have no rows left, no later one has: the sums up to them hold)
+            uint64_t rsum = added;
+            uint32_t nsum = in ? need : 0u;
+            uint64_t tadd;
+            uint32_t tneed;
+            block_scan<T>(rsum, nsum, tadd, tneed);
+            const uint64_t row_end = row0 + rsum;
+            __syncthreads();  // the chunk before has been used
+            s_start[tid] = (uint32_t)(row_end - added);
+            s_len[tid] = len;
+            s_had[tid] = had;
+            s_base[tid] = taken + nsum - (in ? need : 0u);
+            s_added[tid] = added;
+            s_rel[tid] = cr - rel;
+            s_keep[tid] = keep;
+            __syncthreads();
+            if (commit && is) {
+                if (p.added) p.added[b] = added;
+                if (p.row_start) p.row_start[b] = p.rows_per_seq ? b * p.rows_per_seq : (uint32_t)(row_end - added);
+                if (p.row_start && b + 1 == c.n_seqs)
+                    p.row_start[c.n_seqs] = p.rows_per_seq ? c.n_seqs * p.rows_per_seq : (uint32_t)row_end;
+                p.len_out[b] = ends ? 0u : len + added;
+            }
+            if (rows) {
+                const uint32_t nb = min((uint32_t)T, c.n_seqs - b0);
+                const uint32_t r_lo = p.rows_per_seq ? b0 * p.rows_per_seq : (uint32_t)row0;
+                const uint32_t r_hi = p.rows_per_seq ? (b0 + nb) * p.rows_per_seq : (uint32_t)(row0 + tadd);
+                for (uint32_t r = r_lo + blockIdx.x * T + tid; r < r_hi; r += gridDim.x * T) {
+                    const uint32_t i = p.rows_per_seq ? r / p.rows_per_seq - b0 : last_at_or_before(s_start, nb, r);
+                    const uint32_t k = p.rows_per_seq ? r - (b0 + i) * p.rows_per_seq : r - s_start[i];
+                    uint32_t slot = G4A_NO_ROW32, pos = G4A_NO_ROW32;
+                    if (k < s_added[i]) {
+                        pos = s_len[i] + k;
+                        const uint32_t page_no = pos >> shift, e = c.ring ? page_no % P : page_no;
+                        uint32_t* const entry = c.table + (size_t)(b0 + i) * P + e;
+                        uint32_t page;
+                        if (e < s_had[i]) {
+                            page = *entry;
+                        } else {
+                            page = ring_page(s_base[i] + e - s_had[i]);
+                            if ((pos & low) == 0 && page_no < P) *entry = page;
+                        }
+                        // a ring keeps its last tokens: the slots of earlier ones are theirs
+                        const bool kept = !c.ring || (uint64_t)pos + room >= (uint64_t)s_len[i] + s_added[i];
+                        if (kept && page < c.n_pages) slot = (page << shift) + (pos & low);
+                    }
+                    p.slots[r] = slot;
+                    p.positions[r] = pos;
+                }
+                for (uint32_t x = blockIdx.x * T + tid; x < tr; x += gridDim.x * T) {
+                    const uint32_t i = last_at_or_before(s_rel, nb, x);
+                    const uint32_t page = c.table[(size_t)(b0 + i) * P + s_keep[i] + (x - s_rel[i])];
+                    p.free_pages[(uint32_t)(((uint64_t)first + count + rel0 + x) % p.free_cap)] = page;
+                }
+            }
+            row0 += tadd;
+            need0 += tn;
+            rel0 += tr;
+            taken += tneed;
+        }
+        if (rows && p.rows_per_seq == 0)  // rows behind the last sequence
+            for (uint64_t r = row0 + blockIdx.x * T + tid; r < p.rows; r += (uint64_t)gridDim.x * T) {
+                p.slots[r] = G4A_NO_ROW32;
+                p.positions[r] = G4A_NO_ROW32;
+            }
+        if (commit && tid == 0) {
+            p.state_out[0] = (uint32_t)(((uint64_t)first + taken) % p.free_cap);
+            p.state_out[1] = (uint32_t)min((uint64_t)count - taken + rel0, (uint64_t)p.free_cap);
+        }
+    };
+
+    const bool alone = gridDim.x == 1;
+    pass(true, alone || (apart && blockIdx.x == 0));
+    if (alone || apart) return;
+    __syncthreads();  // this workgroup's reads are done
+    if (tid == 0) {
+        __threadfence();
+        s_last = atomicAdd(p.ticket, 1u) == gridDim.x - 1 ? 1u : 0u;
+        if (s_last) *p.ticket = 0u;
+    }
+    __syncthreads();
+    if (s_last) pass(false, true);
+}
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Four values of a page's row, rounded to nearest even where the page holds bf16.
+__device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
+__device__ __forceinline__ void store4(__bf16* p, const f32x4& v) {
+    *reinterpret_cast<bf16x4*>(p) = __builtin_convertvector(v, bf16x4);
+}
+
+// y = rope(x / sqrt(mean(x^2) + eps) * w) for the q, k and v rows of T tokens, in f32: v
+// without w and rotation, q and k unnormalised where w is null. The angle is position *
+// frequency, both f32, as in g4a_norm_rope; its sine and cosine are the device's. The sum
+// of squares is a tree over the row's lanes. K and V rows go to their token's slot.
+//
+// A row takes DH / 4 lanes (two float4 each at 512), so a wave holds 256 / DH of them.
+constexpr int PP_WAVES = 4;
+
+template <int DH, typename KV>
+__device__ __forceinline__ void paged_producer(const G4aPagedProducerParams& p) {
+    constexpr int LPR = DH / 4 < 64 ? DH / 4 : 64;  // lanes of a row
+    constexpr int E = DH / (4 * LPR), RPW = 64 / LPR;
+    __shared__ __attribute__((aligned(16))) float stage[PP_WAVES][RPW][DH + 4];
+    __shared__ float2 turn[PP_WAVES][RPW][DH / 2];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane / LPR, l = lane % LPR;
+    const G4aPaged& c = p.c;
+    const uint64_t row = ((uint64_t)blockIdx.x * PP_WAVES + w) * RPW + g;
+    const bool is = row < (uint64_t)p.T * p.heads;
+    const uint32_t t = is ? (uint32_t)(row / p.heads) : 0u, h = is ? (uint32_t)(row - (uint64_t)t * p.heads) : 0u;
+    const uint32_t pos = is ? p.positions[t] : G4A_NO_ROW32;
+    const uint32_t slot = p.heads > p.Hq && is ? p.slots[t] : G4A_NO_ROW32;
+    const bool on_q = h < p.Hq, on_k = !on_q && h < p.Hq + c.Hkv;
+    const uint32_t kvh = on_q ? 0u : (on_k ? h - p.Hq : h - p.Hq - c.Hkv);
+    const bool live = pos != G4A_NO_ROW32 && (on_q || (slot >> c.page_shift) < c.n_pages);
+    const float* const src = on_q   ? p.q + ((size_t)t * p.Hq + h) * DH
+                             : on_k ? p.kx + ((size_t)t * c.Hkv + kvh) * DH
+                                    : p.vx + ((size_t)t * c.Hkv + kvh) * DH;
+    const float* const wt = on_q ? p.q_norm : on_k ? p.k_norm : nullptr;
+    const bool norm = wt || !(on_q || on_k);
+    f32x4 x[E], wv[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        x[e] = live ? *reinterpret_cast<const f32x4*>(src + 4 * l + 256 * e) : f32x4{0, 0, 0, 0};
+        wv[e] = live && wt ? *reinterpret_cast<const f32x4*>(wt + 4 * l + 256 * e) : f32x4{1, 1, 1, 1};
+    }
+    const uint32_t half = p.rotary_dim / 2;
+    const bool rope = on_q || on_k;
+    if (rope && live)
+        for (uint32_t j = l; j < half; j += LPR) {
+            float sn, cs;
+            sincosf((float)pos * p.freq[j], &sn, &cs);
+            turn[w][g][j] = make_float2(sn, cs);
+        }
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss += (x[e].x * x[e].x + x[e].y * x[e].y) + (x[e].z * x[e].z + x[e].w * x[e].w);
+#pragma unroll
+    for (int d = LPR / 2; d > 0; d >>= 1) ss += __shfl_xor(ss, d);
+    const float inv = norm ? 1.0f / sqrtf(ss / (float)DH + p.eps) : 1.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        x[e] = x[e] * inv * wv[e];
+        *reinterpret_cast<f32x4*>(&stage[w][g][4 * l + 256 * e]) = x[e];
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (!live) return;
+    if (rope)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t d = 4 * l + 256 * e + i;
+                if (d >= p.rotary_dim) continue;
+                const uint32_t j = d < half ? d : d - half;
+                const float a = stage[w][g][j], b = stage[w][g][j + half];
+                const float2 sc = turn[w][g][j];
+                x[e][i] = d < half ? a * sc.y - b * sc.x : b * sc.y + a * sc.x;
+            }
+    if (on_q) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) store4(p.q_out + ((size_t)t * p.Hq + h) * DH + 4 * l + 256 * e, x[e]);
+    } else {
+        KV* const pool = reinterpret_cast<KV*>(on_k ? c.k : c.v);
+        const uint32_t page = slot >> c.page_shift, r = slot & ((1u << c.page_shift) - 1);
+        KV* const dst = pool + (size_t)page * c.page_stride + ((size_t)r * c.Hkv + kvh) * DH;
+#pragma unroll
+        for (int e = 0; e < E; ++e) store4(dst + 4 * l + 256 * e, x[e]);
+    }
+}
+
+// Tokens in order from their pages, as f32. A workgroup copies 1 << rows_shift tokens,
+// which lie on one page, K (blockIdx.y 0) or V: 16 bytes written a thread and step.
+// Tokens the cache does not hold are zeros.
+template <typename KV>
+__device__ __forceinline__ void paged_gather(const G4aPagedGatherParams& p) {
+    typedef KV kv4 __attribute__((ext_vector_type(4)));
+    const G4aPaged& c = p.c;
+    const uint32_t t0 = ((p.pos0 >> p.rows_shift) + blockIdx.x) << p.rows_shift;  // its first token
+    const uint32_t page_no = t0 >> c.page_shift;
+    const uint32_t len = c.len[p.seq];
+    const uint32_t e = c.ring ? page_no % c.per_seq : page_no;
+    const uint32_t page = e < c.per_seq ? c.table[(size_t)p.seq * c.per_seq + e] : c.n_pages;
+    const size_t width = (size_t)c.Hkv * c.Dh;
+    const uint64_t room = (uint64_t)c.per_seq << c.page_shift;
+    // tokens [lo, hi) are asked for, [a, b) of them held
+    const uint64_t lo = max(t0, p.pos0), hi = min((uint64_t)t0 + (1u << p.rows_shift), (uint64_t)p.pos0 + p.n);
+    const uint64_t b = page < c.n_pages ? max(lo, min(hi, (uint64_t)len)) : lo;
+    const uint64_t a = page < c.n_pages && c.ring && len > room ? max(lo, min(b, (uint64_t)len - room)) : lo;
+    float* const out = (blockIdx.y ? p.v_out : p.k_out) + (lo - p.pos0) * width;
+    const KV* const src = reinterpret_cast<const KV*>(blockIdx.y ? c.v : c.k) + (size_t)page * c.page_stride +
+                          (lo & ((1u << c.page_shift) - 1)) * width;
+    const uint32_t n = (uint32_t)((hi - lo) * width / 4), from = (uint32_t)((a - lo) * width / 4),
+                   to = (uint32_t)((b - lo) * width / 4);
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        f32x4 x = {0, 0, 0, 0};
+        if (i >= from && i < to)
+            x = __builtin_convertvector(reinterpret_cast<const kv4*>(src)[i], f32x4);
+        reinterpret_cast<f32x4*>(out)[i] = x;
+    }
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void g4a_page_map_t256(G4aPageMapParams p) { page_map<256>(p); }
+extern "C" __global__ __launch_bounds__(1024) void g4a_page_map_t1024(G4aPageMapParams p) { page_map<1024>(p); }
+#define G4A_PAGED_PRODUCER(dh)                                                                         \
+    extern "C" __global__ __launch_bounds__(256) void g4a_paged_producer_d##dh##_f32(                  \
+        G4aPagedProducerParams p) { paged_producer<dh, float>(p); }                                    \
+    extern "C" __global__ __launch_bounds__(256) void g4a_paged_producer_d##dh##_bf16(                 \
+        G4aPagedProducerParams p) { paged_producer<dh, __bf16>(p); }
+G4A_PAGED_PRODUCER(64) G4A_PAGED_PRODUCER(128) G4A_PAGED_PRODUCER(256) G4A_PAGED_PRODUCER(512)
+#undef G4A_PAGED_PRODUCER
+extern "C" __global__ __launch_bounds__(256) void g4a_paged_gather_f32(G4aPagedGatherParams p) {
+    paged_gather<float>(p);
+}
+extern "C" __global__ __launch_bounds__(256) void g4a_paged_gather_bf16(G4aPagedGatherParams p) {
+    paged_gather<__bf16>(p);
+}

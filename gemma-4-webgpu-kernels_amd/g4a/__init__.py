@@ -24,6 +24,9 @@ HEADER_PATH = PKG_DIR.parent / "include" / "g4a.h"
 G4A_OK = 0
 # G4A_NOALLOC_SCRATCH_BYTES of include/g4a.h: the static scratch of g4a_attention_noalloc
 NOALLOC_SCRATCH_BYTES = 64 << 20
+# g4a_kv_type, G4A_NO_ROW and G4A_SEQ_END of include/g4a.h
+KV_TYPES = {"f32": 0, "bf16": 1}
+NO_ROW = SEQ_END = 0xFFFFFFFF
 KERNEL_NAMES = {0: "none", 1: "decode", 2: "prefill", 3: "generic", 4: "decode_short"}
 
 _u32p = ctypes.POINTER(ctypes.c_uint32)
@@ -73,6 +76,32 @@ class QWeightArgs(ctypes.Structure):
         ("qbytes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("N", ctypes.c_uint32), ("K", ctypes.c_uint32),
         ("bits", ctypes.c_uint32), ("signed_i8", ctypes.c_uint32), ("group_size", ctypes.c_uint32),
     ]
+
+
+class PagedCache(ctypes.Structure):
+    """g4a_paged_cache: pools, tables and widths of a paged KV cache in device memory."""
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("page_stride", ctypes.c_uint64)] + [
+        (n, ctypes.c_uint32) for n in ("n_seqs", "pages_per_seq", "n_pages", "page_size", "Hkv", "Dh", "kv_type", "ring")]
+
+
+class PageMapArgs(ctypes.Structure):
+    """g4a_page_map_args: one step's new tokens and where its slots and positions go."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("new_len", "shared_pages", "free_pages", "free_state", "slots",
+                                               "positions", "row_start", "added", "kv_len_out", "free_state_out")] + [
+        (n, ctypes.c_uint32) for n in ("free_cap", "rows", "rows_per_seq")]
+
+
+class PagedProducerArgs(ctypes.Structure):
+    """g4a_paged_producer_args: T token rows for a paged cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_norm", "k_norm", "q_out", "positions", "slots")] + [
+        (n, ctypes.c_uint32) for n in ("T", "Hq", "rotary_dim")] + [("theta", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """g4a_paged_attn_args: one query of every sequence of a paged cache."""
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("Hq", ctypes.c_uint32),
+                ("sliding_window", ctypes.c_uint32), ("scale", ctypes.c_float), ("attn_softcap", ctypes.c_float)]
 
 
 class DeviceInfo(ctypes.Structure):
@@ -152,6 +181,10 @@ def load_library(path: Path = LIB_PATH) -> ctypes.CDLL:
         "g4a_capture_end": (c_int, [ctxp, ctypes.POINTER(ctypes.c_void_p)]),
         "g4a_graph_launch": (c_int, [ctxp, ctypes.c_void_p]),
         "g4a_graph_destroy": (c_int, [ctypes.c_void_p]),
+        "g4a_page_map": (c_int, [ctxp, ctypes.POINTER(PagedCache), ctypes.POINTER(PageMapArgs)]),
+        "g4a_attn_producer_paged": (c_int, [ctxp, ctypes.POINTER(PagedCache), ctypes.POINTER(PagedProducerArgs)]),
+        "g4a_attention_paged": (c_int, [ctxp, ctypes.POINTER(PagedCache), ctypes.POINTER(PagedAttnArgs)]),
+        "g4a_kv_gather_paged": (c_int, [ctxp, ctypes.POINTER(PagedCache)] + [ctypes.c_uint32] * 3 + [vp, vp]),
         "g4a_timer_start": (c_int, [ctxp]),
         "g4a_timer_stop": (c_int, [ctxp, ctypes.POINTER(ctypes.c_float)]),
         "g4a_get_device_info": (c_int, [ctxp, ctypes.POINTER(DeviceInfo)]),
@@ -460,6 +493,23 @@ class Context:
         arr, ptr = _u32_array(ids)
         n = 0 if arr is None else arr.size
         self._check(self.lib.g4a_embed_rows_q(self.handle, ctypes.byref(table.args), ptr, n, scale, out))
+
+    # ---- paged KV cache (argument blocks are filled once and reused) ----
+    def page_map(self, cache: PagedCache, args: PageMapArgs) -> None:
+        """g4a_page_map: the pages, slots and positions of one step, from lengths on the device."""
+        self._check(self.lib.g4a_page_map(self.handle, cache, args))
+
+    def attn_producer_paged(self, cache: PagedCache, args: PagedProducerArgs) -> None:
+        """g4a_attn_producer_paged: norm and RoPE of q, k and v, K and V into the tokens' slots."""
+        self._check(self.lib.g4a_attn_producer_paged(self.handle, cache, args))
+
+    def attention_paged(self, cache: PagedCache, args: PagedAttnArgs) -> None:
+        """g4a_attention_paged: one query of every sequence over its tokens in the cache."""
+        self._check(self.lib.g4a_attention_paged(self.handle, cache, args))
+
+    def kv_gather_paged(self, cache: PagedCache, seq: int, pos0: int, n: int, k_out: int, v_out: int) -> None:
+        """g4a_kv_gather_paged: tokens pos0 .. pos0 + n - 1 of a sequence in order, as f32 rows."""
+        self._check(self.lib.g4a_kv_gather_paged(self.handle, cache, seq, pos0, n, k_out, v_out))
 
     # ---- graph capture (launch-bound sequences) ----
     def capture_begin(self) -> None:

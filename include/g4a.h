@@ -470,6 +470,138 @@ int g4a_attention_devpos(g4a_ctx *ctx, const g4a_attn_args *args, const uint32_t
 int g4a_attn_producer_devpos(g4a_ctx *ctx, const g4a_producer_args *args, const uint32_t *pos, uint32_t max_pos);
 int g4a_u32_add(g4a_ctx *ctx, uint32_t *counters, uint32_t n, uint32_t inc);
 
+/* ---- paged KV cache -------------------------------------------------------
+ * No counterpart in the reference, whose cache is one growing buffer a layer
+ * (rust/src/kvcache.rs:49-62): the cache of a server, where sequences share a
+ * pool of pages, with every length, table and position in device memory, so that
+ * a whole decode step (g4a_page_map, then per layer g4a_attn_producer_paged and
+ * g4a_attention_paged) captures into a graph once and replays as the sequences
+ * grow, end and start.
+ *
+ * Token t of sequence b is row t % page_size of page
+ * block_table[b * pages_per_seq + t / page_size]; with `ring` the table is a ring
+ * (entry t / page_size % pages_per_seq) that holds a sequence's last
+ * pages_per_seq * page_size tokens, as a sliding layer needs. A page is page_size
+ * rows of [Hkv, Dh] values, K and V in pools of their own; an entry of n_pages or
+ * more names no page, and tokens on it are treated as absent. Layers that share
+ * tables and lengths differ in their pools alone. Pages may be shared between
+ * sequences (a common prefix) as long as nobody writes into them.
+ *
+ * All of these return G4A_E_ARG on null or misaligned pointers and values out of
+ * range, G4A_E_SHAPE on shapes that do not fit each other and
+ * G4A_E_UNSUPPORTED on others; what stands in device memory is not checked by the
+ * host, and no value there makes a kernel read or write outside the buffers
+ * described here (a token whose slot or page does not exist is left out). */
+#define G4A_NO_ROW 0xFFFFFFFFu  /* no slot, no position */
+#define G4A_SEQ_END 0xFFFFFFFFu /* in new_len: the sequence ends */
+
+typedef enum g4a_kv_type {
+    G4A_KV_F32 = 0,
+    G4A_KV_BF16 = 1, /* rounded to nearest even on writing; every operator computes in f32 */
+} g4a_kv_type;
+
+typedef struct g4a_paged_cache {
+    void *k_pages;         /* device, 16-byte aligned */
+    void *v_pages;
+    uint32_t *block_table; /* device [n_seqs, pages_per_seq] */
+    uint32_t *kv_len;      /* device [n_seqs]: tokens of each sequence */
+    uint64_t page_stride;  /* values from one page to the next, a multiple of 8; 0: page_size * Hkv * Dh */
+    uint32_t n_seqs, pages_per_seq;
+    uint32_t n_pages;      /* n_pages * page_size < 2^32 */
+    uint32_t page_size;    /* tokens, a power of two from 16 to 65536 */
+    uint32_t Hkv;          /* at most 1024 */
+    uint32_t Dh;           /* 64, 128, 256 or 512 */
+    uint32_t kv_type;      /* g4a_kv_type */
+    uint32_t ring;         /* 0, or 1: the tables are rings */
+} g4a_paged_cache;
+
+/* The pages, slots and positions of one step, from lengths on the device.
+ * Sequence b (kv_len[b] tokens so far) adds new_len[b] tokens: pages it lacks are
+ * taken from the free ring in order and entered in its table, and token i of it,
+ * at position kv_len[b] + i, gets the slot page * page_size + row that
+ * g4a_attn_producer_paged writes to. With rows_per_seq = 0 the tokens' rows are
+ * packed, sequence after sequence, from row 0 on; else sequence b's are rows
+ * b * rows_per_seq onwards (rows = n_seqs * rows_per_seq; a batch of fixed size,
+ * one row each in a decode step). A row without a token gets slot and position
+ * G4A_NO_ROW; so does the slot of a token that a ring loses within the step.
+ *
+ * A sequence adds all of its tokens or none. None: if they do not fit its table
+ * (linear) or rows_per_seq, if it needs pages and the running sum of the pages
+ * needed so far, in sequence order, passes the free ones, or, packed, if the
+ * running sum of rows passes `rows`. added[b] says how many it got. A sequence of
+ * new_len G4A_SEQ_END ends: its pages, but for the first shared_pages[b], go to
+ * the end of the free ring in table order (for the next call) and its length
+ * becomes 0.
+ *
+ * free_pages is a ring of free_cap page numbers, free_state its {first, count};
+ * free_cap must hold all pages that can be free at once. kv_len_out and
+ * free_state_out receive the lengths and the state after the step, NULL:
+ * cache->kv_len and free_state themselves; table and ring are written in place.
+ * The cache's pools and widths are not looked at. */
+typedef struct g4a_page_map_args {
+    const uint32_t *new_len;      /* device [n_seqs], or NULL: one token each */
+    const uint32_t *shared_pages; /* device [n_seqs], or NULL: none */
+    uint32_t *free_pages;         /* device [free_cap] */
+    uint32_t *free_state;         /* device [2] */
+    uint32_t *slots;              /* device [rows] */
+    uint32_t *positions;          /* device [rows] */
+    uint32_t *row_start;          /* device [n_seqs + 1], or NULL: first row of each sequence, and the end */
+    uint32_t *added;              /* device [n_seqs], or NULL */
+    uint32_t *kv_len_out;         /* device [n_seqs], or NULL */
+    uint32_t *free_state_out;     /* device [2], or NULL */
+    uint32_t free_cap;
+    uint32_t rows;                /* below 2^31 */
+    uint32_t rows_per_seq;
+} g4a_page_map_args;
+
+int g4a_page_map(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4a_page_map_args *args);
+
+/* g4a_attn_producer for T token rows at positions and slots in device memory (as
+ * g4a_page_map writes them): q_out = rope(norm(q)), and K = rope(norm(k)) and
+ * V = norm(v) into the token's slot. The rotation's angle is position * frequency
+ * in f32 as there; sums and sines are the device's, so values agree with that
+ * call's to f32 rounding. A row at position G4A_NO_ROW is left alone, q_out
+ * included; slot G4A_NO_ROW (or one past the pool) writes no K and V. The slots
+ * of a call differ from each other. k = v = NULL: only q. Of the cache the pools
+ * and widths are used. A (theta, rotary_dim) pair's first use must be outside a
+ * capture. */
+typedef struct g4a_paged_producer_args {
+    const float *q;      /* [T, Hq, Dh], 16-byte aligned like all rows here */
+    const float *k;      /* [T, Hkv, Dh], or NULL */
+    const float *v;      /* [T, Hkv, Dh], or NULL */
+    const float *q_norm; /* [Dh], or NULL: rotation only */
+    const float *k_norm; /* [Dh], or NULL: rotation only */
+    float *q_out;        /* [T, Hq, Dh], may be q */
+    const uint32_t *positions; /* device [T] */
+    const uint32_t *slots;     /* device [T]; may be NULL when k is */
+    uint32_t T, Hq, rotary_dim;
+    float theta, eps;
+} g4a_paged_producer_args;
+
+int g4a_attn_producer_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4a_paged_producer_args *args);
+
+/* Attention of one query of every sequence over its tokens in the cache: the
+ * query of sequence b sits at position kv_len[b] - 1 and sees the last
+ * sliding_window tokens (0: all; a ring: at most those it holds), with scale and
+ * soft-cap as in g4a_attention; zeros where kv_len[b] is 0. Query head h reads kv
+ * head h / (Hq / Hkv). Every kernel and grid depends on the arguments alone, so a
+ * captured call follows lengths and tables. */
+typedef struct g4a_paged_attn_args {
+    const float *q; /* [n_seqs, Hq, Dh], 16-byte aligned */
+    float *out;     /* [n_seqs, Hq * Dh], 16-byte aligned */
+    uint32_t Hq;
+    uint32_t sliding_window;
+    float scale, attn_softcap;
+} g4a_paged_attn_args;
+
+int g4a_attention_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4a_paged_attn_args *args);
+
+/* Tokens pos0 .. pos0 + n - 1 of sequence `seq` in order, as f32 rows [n, Hkv, Dh]:
+ * a cached prefix for g4a_attention over a prompt that continues it. Tokens the
+ * cache does not hold (past kv_len[seq], lost by a ring, on no page) are zeros. */
+int g4a_kv_gather_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, uint32_t seq, uint32_t pos0, uint32_t n,
+                        float *k_out, float *v_out);
+
 /* ---- timing (HIP events on the context's stream) ----------------------- */
 int g4a_timer_start(g4a_ctx *ctx);
 /* Records the stop event, waits for it and returns the elapsed milliseconds. */

@@ -1,0 +1,159 @@
+"""The paged KV cache's entry points on the host side of the library, over a stand-in
+for the HIP runtime: what they refuse, with which code, and that a refused call
+launches nothing; which kernels the others launch. CPU only."""
+import numpy as np
+import pytest
+
+import hip_standin as hip
+import paged_ref as ref
+from hip_standin import PTR
+
+ARG, SHAPE, UNSUPPORTED = -2, -3, -4
+
+
+@pytest.fixture
+def ctx():
+    c = hip.binding().Context(0)
+    hip.launches()
+    yield c
+    c.close()
+
+
+def _cache(**kw):
+    base = dict(k_pages=PTR, v_pages=PTR, block_table=PTR, kv_len=PTR, n_seqs=4, pages_per_seq=8, n_pages=64,
+                page_size=16, Hkv=1, Dh=256, kv_type=0, ring=0)
+    base.update(kw)
+    return hip.binding().PagedCache(**base)
+
+
+def _map(**kw):
+    base = dict(free_pages=PTR, free_state=PTR, slots=PTR, positions=PTR, free_cap=64, rows=100)
+    base.update(kw)
+    return hip.binding().PageMapArgs(**base)
+
+
+def _producer(**kw):
+    base = dict(q=PTR, k=PTR, v=PTR, q_norm=PTR, k_norm=PTR, q_out=PTR, positions=PTR, slots=PTR, T=3, Hq=8,
+                rotary_dim=256, theta=1e4, eps=1e-6)
+    base.update(kw)
+    return hip.binding().PagedProducerArgs(**base)
+
+
+def _attn(**kw):
+    base = dict(q=PTR, out=PTR, Hq=8, scale=1.0)
+    base.update(kw)
+    return hip.binding().PagedAttnArgs(**base)
+
+
+def _refused(ctx, code, text, call, *args):
+    with pytest.raises(hip.binding().G4aError) as e:
+        call(*args)
+    assert e.value.code == code and text in str(e.value), str(e.value)
+    assert hip.launches() == []
+
+
+POOLS = [
+    (UNSUPPORTED, "page_size", dict(page_size=8)), (UNSUPPORTED, "page_size", dict(page_size=48)),
+    (UNSUPPORTED, "page_size", dict(page_size=1 << 17)), (UNSUPPORTED, "page_size", dict(page_size=0)),
+    (SHAPE, "slots", dict(n_pages=0)), (SHAPE, "slots", dict(n_pages=1 << 28, page_size=16)),
+    (ARG, "ring", dict(ring=2)), (UNSUPPORTED, "head_dim", dict(Dh=96)), (UNSUPPORTED, "head_dim", dict(Dh=0)),
+    (UNSUPPORTED, "Hkv", dict(Hkv=0)), (UNSUPPORTED, "Hkv", dict(Hkv=2000)), (ARG, "kv_type", dict(kv_type=2)),
+    (ARG, "k_pages", dict(k_pages=None)), (ARG, "v_pages", dict(v_pages=PTR + 8)),
+    (SHAPE, "page_stride", dict(page_stride=16 * 256 - 8)), (SHAPE, "page_stride", dict(page_stride=16 * 256 + 4)),
+    (SHAPE, "page_stride", dict(page_stride=1 << 41)),
+]
+TABLES = [
+    (ARG, "block_table", dict(block_table=None)), (ARG, "kv_len", dict(kv_len=None)),
+    (SHAPE, "tables", dict(pages_per_seq=0)), (SHAPE, "tables", dict(pages_per_seq=1 << 28)),
+    (SHAPE, "tables", dict(n_seqs=1 << 31, pages_per_seq=2)),
+]
+
+
+@pytest.mark.parametrize("code,text,kw", POOLS + TABLES)
+def test_bad_caches_are_refused(ctx, code, text, kw):
+    if text not in ("slots", "page_size", "ring") and (code, text, kw) not in TABLES:  # what page_map does not look at
+        ctx.page_map(_cache(**kw), _map())
+        assert len(hip.launches()) == 1
+    else:
+        _refused(ctx, code, text, ctx.page_map, _cache(**kw), _map())
+    if (code, text, kw) not in TABLES:  # the producer looks at pools alone
+        _refused(ctx, code, text, ctx.attn_producer_paged, _cache(**kw), _producer())
+    _refused(ctx, code, text, ctx.attention_paged, _cache(**kw), _attn())
+    _refused(ctx, code, text, ctx.kv_gather_paged, _cache(**kw), 0, 0, 5, PTR, PTR)
+
+
+@pytest.mark.parametrize("code,text,kw", [
+    (ARG, "slots", dict(slots=None)), (ARG, "positions", dict(positions=None)), (ARG, "free", dict(free_pages=None)),
+    (ARG, "free", dict(free_state=None)), (ARG, "free", dict(free_cap=0)), (SHAPE, "rows", dict(rows=1 << 31)),
+    (SHAPE, "rows", dict(rows_per_seq=1)),
+])
+def test_bad_maps_are_refused(ctx, code, text, kw):
+    _refused(ctx, code, text, ctx.page_map, _cache(), _map(**kw))
+
+
+@pytest.mark.parametrize("code,text,kw", [
+    (ARG, "rotary_dim", dict(rotary_dim=3)), (ARG, "rotary_dim", dict(rotary_dim=258)), (ARG, "k and v", dict(k=None)),
+    (UNSUPPORTED, "Hq", dict(Hq=0)), (SHAPE, "rows", dict(T=1 << 31)), (ARG, "null", dict(q=None)),
+    (ARG, "null", dict(q_out=None)), (ARG, "null", dict(positions=None)), (ARG, "null", dict(slots=None)),
+    (ARG, "aligned", dict(q=PTR + 4)), (ARG, "aligned", dict(k_norm=PTR + 8)),
+])
+def test_bad_producers_are_refused(ctx, code, text, kw):
+    _refused(ctx, code, text, ctx.attn_producer_paged, _cache(), _producer(**kw))
+
+
+@pytest.mark.parametrize("code,text,cache,kw", [
+    (SHAPE, "Hq", {}, dict(Hq=0)), (SHAPE, "Hq", dict(Hkv=3), dict(Hq=8)), (SHAPE, "Hq", {}, dict(Hq=1 << 17)),
+    (ARG, "softcap", {}, dict(attn_softcap=-1.0)), (ARG, "softcap", {}, dict(attn_softcap=float("nan"))),
+    (ARG, "null", {}, dict(q=None)), (ARG, "aligned", {}, dict(out=PTR + 4)),
+])
+def test_bad_attention_calls_are_refused(ctx, code, text, cache, kw):
+    _refused(ctx, code, text, ctx.attention_paged, _cache(**cache), _attn(**kw))
+
+
+@pytest.mark.parametrize("code,text,args", [
+    (ARG, "sequence", (4, 0, 5, PTR, PTR)), (SHAPE, "positions", (0, 0xFFFFFFF0, 32, PTR, PTR)),
+    (ARG, "null", (0, 0, 5, None, PTR)), (ARG, "aligned", (0, 0, 5, PTR, PTR + 4)),
+])
+def test_bad_gathers_are_refused(ctx, code, text, args):
+    _refused(ctx, code, text, ctx.kv_gather_paged, _cache(), *args)
+
+
+def test_calls_without_work_launch_nothing(ctx):
+    ctx.page_map(_cache(n_seqs=0), _map(rows=0))
+    ctx.attn_producer_paged(_cache(), _producer(T=0))
+    ctx.attention_paged(_cache(n_seqs=0), _attn())
+    ctx.kv_gather_paged(_cache(), 0, 7, 0, PTR, PTR)
+    assert hip.launches() == []
+
+
+def test_a_rotation_is_first_used_outside_a_capture(ctx):
+    ctx.capture_begin()
+    with pytest.raises(hip.binding().G4aError, match="capture"):
+        ctx.attn_producer_paged(_cache(), _producer(theta=777.0))
+    with pytest.raises(hip.binding().G4aError):
+        ctx.capture_end()
+    ctx.attn_producer_paged(_cache(), _producer(theta=777.0))
+    ctx.capture_begin()
+    ctx.page_map(_cache(), _map(rows=4, rows_per_seq=1))
+    ctx.attn_producer_paged(_cache(), _producer(theta=777.0))
+    ctx.attention_paged(_cache(), _attn())
+    ctx.kv_gather_paged(_cache(), 0, 0, 5, PTR, PTR)
+    ctx.capture_end().free()
+
+
+def test_the_reference_map_keeps_every_page_once():
+    """Steps of random demands: pages are owned by one sequence or free, never both, and
+    slots of live tokens differ."""
+    rng = np.random.default_rng(5)
+    n, per_seq, page, cap = 6, 4, 16, 20
+    lens, table = np.zeros(n, np.uint32), np.full((n, per_seq), ref.NO_ROW, np.uint32)
+    free, first, count = rng.permutation(cap).astype(np.uint32), 3, cap
+    for _ in range(60):
+        new = np.where(rng.random(n) < 0.15, ref.NO_ROW, rng.integers(0, 30, n)).astype(np.uint32)
+        slots, pos, start, added, lens, table, free, first, count = ref.page_map(
+            lens, new, table, free, first, count, page=page, ring=False, rows=64)
+        owned = [p for b in range(n) for p in table[b, :-(-int(lens[b]) // page)]]
+        left = [free[(first + i) % cap] for i in range(count)]
+        assert sorted(owned + left) == list(range(cap))
+        live = slots[slots != ref.NO_ROW]
+        assert len(set(live)) == len(live) == added.sum() == start[n]
