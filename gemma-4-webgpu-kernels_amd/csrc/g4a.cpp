@@ -99,6 +99,10 @@ struct g4a_graph_book {
     std::vector<void*> retired;  // workspaces replaced while graphs were live
 };
 
+// Most query heads of a unit of the paged decode: 16 at head_dim 512 over f32 pages
+// would take more registers than there are.
+static uint32_t paged_most_heads(uint32_t Dh, int kv_type) { return Dh == 512 && kv_type == G4A_KV_F32 ? 8 : 16; }
+
 struct g4a_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
@@ -154,7 +158,8 @@ struct g4a_ctx {
     // the paged KV cache: [head_dim 64, 128, 256, 512][f32, bf16 pages]
     hipFunction_t page_map[2] = {};  // [256, 1024 threads]
     hipFunction_t paged_producer[4][2] = {};
-    hipFunction_t paged_decode[4][2] = {};
+    hipFunction_t paged_decode[4][2][3] = {};  // [4, 8, 16 heads a unit]
+    hipFunction_t paged_combine[4][2][3] = {};
     hipFunction_t paged_gather[2] = {};
     uint32_t* ticket = nullptr;  // g4a_page_map's: 0 between launches
     // RoPE frequency tables theta^(-2j/rot), one per (theta, rotary_dim) seen
@@ -913,8 +918,12 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
         for (int d = 0; d < 4; ++d) {
             snprintf(name, sizeof name, "g4a_paged_producer_d%d_%s", 64 << d, type);
             if (int rc = get_fn(ctx, &ctx->paged_producer[d][t], name)) return bail(rc);
-            snprintf(name, sizeof name, "g4a_paged_decode_d%d_%s", 64 << d, type);
-            if (int rc = get_fn(ctx, &ctx->paged_decode[d][t], name)) return bail(rc);
+            for (int h = 0; h < (paged_most_heads(64u << d, t) == 16 ? 3 : 2); ++h) {
+                snprintf(name, sizeof name, "g4a_paged_decode_d%d_%s_h%d", 64 << d, type, 1 << h);
+                if (int rc = get_fn(ctx, &ctx->paged_decode[d][t][h], name)) return bail(rc);
+                snprintf(name, sizeof name, "g4a_paged_combine_d%d_%s_h%d", 64 << d, type, 1 << h);
+                if (int rc = get_fn(ctx, &ctx->paged_combine[d][t][h], name)) return bail(rc);
+            }
         }
         snprintf(name, sizeof name, "g4a_paged_gather_%s", type);
         if (int rc = get_fn(ctx, &ctx->paged_gather[t], name)) return bail(rc);
@@ -2318,6 +2327,12 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Fewest tiles (16 tokens) of a workgroup of the paged decode.
+constexpr uint32_t PAGED_MIN_RUN = 4;
+// Its workgroups per CU: [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
+constexpr uint32_t PAGED_WGS_PER_CU[4][2][3] = {
+    {{4, 3, 2}, {4, 2, 1}}, {{3, 2, 2}, {4, 2, 1}}, {{2, 2, 1}, {3, 2, 1}}, {{1, 1, 0}, {2, 1, 1}}};
+
 // Index of a paged cache's head_dim among the kernels'.
 int paged_dh(uint32_t Dh) { return Dh == 64 ? 0 : Dh == 128 ? 1 : Dh == 256 ? 2 : 3; }
 
@@ -2444,11 +2459,33 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.q = a->q;
     p.out = a->out;
     p.Hq = a->Hq;
-    p.window = a->sliding_window;
+    const uint64_t room = uint64_t(cache->pages_per_seq) * cache->page_size;
+    p.room = uint32_t(room);
+    p.span = a->sliding_window ? std::min(a->sliding_window, p.room) : p.room;
+    p.group = a->Hq / cache->Hkv;
+    const int h = p.group <= 4 ? 0 : p.group <= 8 || paged_most_heads(cache->Dh, cache->kv_type) == 8 ? 1 : 2;
+    const uint32_t heads = 4u << h;
+    p.chunks = (p.group + heads - 1) / heads;
+    p.units = cache->Hkv * p.chunks;
+    const size_t item = size_t(heads) * cache->Dh;
+    const uint32_t blocks = uint32_t(item / 4 / 16);  // of a unit's merge
+    if (std::max<uint64_t>(p.span / 16 + 2, blocks) * cache->n_seqs * p.units >> 31)
+        return fail(ctx, G4A_E_SHAPE, "%u sequences of up to %u tokens in %u head groups: at most 2^31 tiles of 16 tokens",
+                    cache->n_seqs, p.span, p.units);
+    p.min_run = PAGED_MIN_RUN;
     p.scale = a->scale;
     p.softcap = a->attn_softcap;
-    return launch(ctx, ctx->paged_decode[paged_dh(cache->Dh)][cache->kv_type], dim3(cache->n_seqs, a->Hq, 1),
-                  dim3(256, 1, 1), p, "paged decode", true);
+    const int d = paged_dh(cache->Dh), t = int(cache->kv_type);
+    const uint32_t wgs = uint32_t(std::max(ctx->cu_count, 1)) * PAGED_WGS_PER_CU[d][t][h];
+    const size_t offs = (size_t(cache->n_seqs) + 1 + 63) / 64 * 64;
+    if (int rc = ensure_workspace(ctx, (offs + size_t(2) * wgs * (item + 2 * heads)) * sizeof(float))) return rc;
+    p.offs = static_cast<uint32_t*>(ctx->workspace);
+    p.part = static_cast<float*>(ctx->workspace) + offs;
+    p.part_ml = p.part + size_t(2) * wgs * item;
+    if (int rc = launch(ctx, ctx->paged_decode[d][t][h], dim3(wgs, 1, 1), dim3(256, 1, 1), p, "paged decode", true))
+        return rc;
+    return launch(ctx, ctx->paged_combine[d][t][h], dim3(blocks * cache->n_seqs * p.units, 1, 1), dim3(256, 1, 1), p,
+                  "paged combine", true);
 }
 
 int g4a_kv_gather_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, uint32_t seq, uint32_t pos0, uint32_t n,

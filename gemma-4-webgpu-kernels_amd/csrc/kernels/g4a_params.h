@@ -401,11 +401,21 @@ struct G4aPagedGatherParams {
     uint32_t rows_shift;     // log2 of the tokens of a workgroup (within one page)
 };
 
-// One query of every sequence over its pages (g4a_paged_decode_*).
+// One query of every sequence over its pages (g4a_paged_decode_*, g4a_paged_combine_*).
+// A unit is 4, 8 or 16 heads (the kernel's) of one kv head's group; a sequence has
+// units = Hkv * chunks of them.
 struct G4aPagedAttnParams {
     G4aPaged c;
     const float* q;          // [n_seqs, Hq, Dh]
     float* out;              // [n_seqs, Hq * Dh]
-    uint32_t Hq, window;
+    uint32_t Hq, group, chunks, units;
+    uint32_t room, span;     // tokens a sequence's table holds, most a query sees
+    uint32_t min_run;        // fewest tiles of a workgroup's run
     float scale, softcap;
+    // written by the decode kernel, read by the combine: offs[0] tiles of a run, offs[1 + b]
+    // first tile of sequence b; two partial slots a workgroup: O in the accumulators' order
+    // and (m, l) of each head
+    uint32_t* offs;
+    float* part;
+    float* part_ml;
 };

@@ -133,6 +133,7 @@ def test_a_rotation_is_first_used_outside_a_capture(ctx):
     with pytest.raises(hip.binding().G4aError):
         ctx.capture_end()
     ctx.attn_producer_paged(_cache(), _producer(theta=777.0))
+    ctx.attention_paged(_cache(), _attn())  # (and its workspace)
     ctx.capture_begin()
     ctx.page_map(_cache(), _map(rows=4, rows_per_seq=1))
     ctx.attn_producer_paged(_cache(), _producer(theta=777.0))
