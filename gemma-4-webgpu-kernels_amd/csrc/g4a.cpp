@@ -158,8 +158,8 @@ struct g4a_ctx {
     // the paged KV cache: [head_dim 64, 128, 256, 512][f32, bf16 pages]
     hipFunction_t page_map[2] = {};  // [256, 1024 threads]
     hipFunction_t paged_producer[4][2] = {};
-    hipFunction_t paged_decode[4][2][3] = {};  // [4, 8, 16 heads a unit]
-    hipFunction_t paged_combine[4][2][3] = {};
+    hipFunction_t paged_decode[2][4][2][3] = {};  // [whole context, window] ... [4, 8, 16 heads a unit]
+    hipFunction_t paged_combine[2][4][2][3] = {};  // [16, 64 items a block] ...
     hipFunction_t paged_gather[2] = {};
     uint32_t* ticket = nullptr;  // g4a_page_map's: 0 between launches
     // RoPE frequency tables theta^(-2j/rot), one per (theta, rotary_dim) seen
@@ -919,10 +919,14 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
             snprintf(name, sizeof name, "g4a_paged_producer_d%d_%s", 64 << d, type);
             if (int rc = get_fn(ctx, &ctx->paged_producer[d][t], name)) return bail(rc);
             for (int h = 0; h < (paged_most_heads(64u << d, t) == 16 ? 3 : 2); ++h) {
-                snprintf(name, sizeof name, "g4a_paged_decode_d%d_%s_h%d", 64 << d, type, 1 << h);
-                if (int rc = get_fn(ctx, &ctx->paged_decode[d][t][h], name)) return bail(rc);
-                snprintf(name, sizeof name, "g4a_paged_combine_d%d_%s_h%d", 64 << d, type, 1 << h);
-                if (int rc = get_fn(ctx, &ctx->paged_combine[d][t][h], name)) return bail(rc);
+                for (int win = 0; win < 2; ++win) {
+                    snprintf(name, sizeof name, "g4a_paged_decode%s_d%d_%s_h%d", win ? "_win" : "", 64 << d, type, 1 << h);
+                    if (int rc = get_fn(ctx, &ctx->paged_decode[win][d][t][h], name)) return bail(rc);
+                }
+                for (int w = 0; w < 2; ++w) {
+                    snprintf(name, sizeof name, "g4a_paged_combine%d_d%d_%s_h%d", w ? 64 : 16, 64 << d, type, 1 << h);
+                    if (int rc = get_fn(ctx, &ctx->paged_combine[w][d][t][h], name)) return bail(rc);
+                }
             }
         }
         snprintf(name, sizeof name, "g4a_paged_gather_%s", type);
@@ -2327,8 +2331,14 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Fewest tiles (16 tokens) of a workgroup of the paged decode.
-constexpr uint32_t PAGED_MIN_RUN = 4;
+// Fewest tiles (16 tokens) of a part of the paged decode: one for each wave.
+constexpr uint32_t PAGED_MIN_PART = 4;
+// Most parts of a unit: the merge keeps a weight for each (attn_paged.hip).
+constexpr uint32_t PAGED_MAX_PARTS = 1024;
+// Units up to which a merge block takes 16 items of one, not 64.
+constexpr uint32_t PAGED_FEW_UNITS = 8;
+// Most units of a launch (but for a sequence that has more).
+constexpr uint32_t PAGED_UNITS = 2048;
 // Its workgroups per CU: [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
 constexpr uint32_t PAGED_WGS_PER_CU[4][2][3] = {
     {{4, 3, 2}, {4, 2, 1}}, {{3, 2, 2}, {4, 2, 1}}, {{2, 2, 1}, {3, 2, 1}}, {{1, 1, 0}, {2, 1, 1}}};
@@ -2468,24 +2478,49 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.chunks = (p.group + heads - 1) / heads;
     p.units = cache->Hkv * p.chunks;
     const size_t item = size_t(heads) * cache->Dh;
-    const uint32_t blocks = uint32_t(item / 4 / 16);  // of a unit's merge
-    if (std::max<uint64_t>(p.span / 16 + 2, blocks) * cache->n_seqs * p.units >> 31)
+    if (std::max<uint64_t>(p.span / 16 + 2, item / 64) * cache->n_seqs * p.units >> 31)
         return fail(ctx, G4A_E_SHAPE, "%u sequences of up to %u tokens in %u head groups: at most 2^31 tiles of 16 tokens",
                     cache->n_seqs, p.span, p.units);
-    p.min_run = PAGED_MIN_RUN;
+    p.min_part = PAGED_MIN_PART;
     p.scale = a->scale;
     p.softcap = a->attn_softcap;
     const int d = paged_dh(cache->Dh), t = int(cache->kv_type);
-    const uint32_t wgs = uint32_t(std::max(ctx->cu_count, 1)) * PAGED_WGS_PER_CU[d][t][h];
-    const size_t offs = (size_t(cache->n_seqs) + 1 + 63) / 64 * 64;
-    if (int rc = ensure_workspace(ctx, (offs + size_t(2) * wgs * (item + 2 * heads)) * sizeof(float))) return rc;
+    const uint32_t resident = uint32_t(std::max(ctx->cu_count, 1)) * PAGED_WGS_PER_CU[d][t][h];
+    // launches of at most PAGED_UNITS units, which bounds the partials' memory
+    const uint32_t most = std::min(cache->n_seqs, std::max(1u, PAGED_UNITS / p.units));
+    // parts: as many as the GPU runs at once, no more of units that leave room for a few parts each, and else
+    // about as many again; none of fewer tiles than there are
+    auto shares = [&](uint32_t seqs, uint32_t* spread, uint32_t* fit) {
+        const uint64_t units = uint64_t(seqs) * p.units, tiles = uint64_t(p.span / 16 + 2) * units;
+        const uint64_t most_parts = std::min<uint64_t>(std::min(resident, PAGED_MAX_PARTS), tiles / PAGED_MIN_PART + units);
+        *fit = 2 * units <= most_parts ? uint32_t(most_parts) : 0;
+        *spread = uint32_t(std::max<uint64_t>(1, *fit ? most_parts : std::min<uint64_t>(resident, PAGED_MAX_PARTS - 1)));
+        return *fit ? *fit : uint32_t(*spread + units);  // the workgroups
+    };
+    uint32_t slots = shares(most, &p.spread, &p.fit);
+    if (cache->n_seqs % most) slots = std::max(slots, shares(cache->n_seqs % most, &p.spread, &p.fit));
+    const size_t offs = (size_t(most) + 1 + 63) / 64 * 64;
+    if (int rc = ensure_workspace(ctx, (offs + slots * (item + 2 * heads)) * sizeof(float))) return rc;
     p.offs = static_cast<uint32_t*>(ctx->workspace);
     p.part = static_cast<float*>(ctx->workspace) + offs;
-    p.part_ml = p.part + size_t(2) * wgs * item;
-    if (int rc = launch(ctx, ctx->paged_decode[d][t][h], dim3(wgs, 1, 1), dim3(256, 1, 1), p, "paged decode", true))
-        return rc;
-    return launch(ctx, ctx->paged_combine[d][t][h], dim3(blocks * cache->n_seqs * p.units, 1, 1), dim3(256, 1, 1), p,
-                  "paged combine", true);
+    p.part_ml = p.part + size_t(slots) * item;
+    const G4aPagedAttnParams all = p;
+    for (uint32_t b0 = 0; b0 < cache->n_seqs; b0 += most) {
+        p.c.n_seqs = std::min(most, cache->n_seqs - b0);
+        p.c.table = all.c.table + size_t(b0) * cache->pages_per_seq;
+        p.c.len = all.c.len + b0;
+        p.q = all.q + size_t(b0) * a->Hq * cache->Dh;
+        p.out = all.out + size_t(b0) * a->Hq * cache->Dh;
+        const uint32_t wgs = shares(p.c.n_seqs, &p.spread, &p.fit), units = p.c.n_seqs * p.units;
+        if (int rc = launch(ctx, ctx->paged_decode[a->sliding_window != 0][d][t][h], dim3(wgs, 1, 1), dim3(256, 1, 1), p,
+                            "paged decode", true))
+            return rc;
+        const uint32_t wide = units > PAGED_FEW_UNITS, blocks = uint32_t(item / 4) / (wide ? 64 : 16);
+        if (int rc = launch(ctx, ctx->paged_combine[wide][d][t][h], dim3(blocks * units, 1, 1), dim3(256, 1, 1), p,
+                            "paged combine", true))
+            return rc;
+    }
+    return G4A_OK;
 }
 
 int g4a_kv_gather_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, uint32_t seq, uint32_t pos0, uint32_t n,

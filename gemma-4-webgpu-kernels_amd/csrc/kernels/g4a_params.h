@@ -410,11 +410,13 @@ struct G4aPagedAttnParams {
     float* out;              // [n_seqs, Hq * Dh]
     uint32_t Hq, group, chunks, units;
     uint32_t room, span;     // tokens a sequence's table holds, most a query sees
-    uint32_t min_run;        // fewest tiles of a workgroup's run
+    uint32_t spread;         // a part's tiles are about all over this many
+    uint32_t fit;            // parts there may be at most, or 0: spread + one a unit
+    uint32_t min_part;       // tiles of a part, at least (of a unit that has as many)
     float scale, softcap;
-    // written by the decode kernel, read by the combine: offs[0] tiles of a run, offs[1 + b]
-    // first tile of sequence b; two partial slots a workgroup: O in the accumulators' order
-    // and (m, l) of each head
+    // written by the decode kernel, read by the combine: offs[0] most tiles of a part, offs[1 + b]
+    // first part of sequence b; a slot a workgroup: O in the accumulators' order, and the heads'
+    // maxima, then their sums
     uint32_t* offs;
     float* part;
     float* part_ml;
