@@ -99,10 +99,6 @@ struct g4a_graph_book {
     std::vector<void*> retired;  // workspaces replaced while graphs were live
 };
 
-// Most query heads of a unit of the paged decode: 16 at head_dim 512 over f32 pages
-// would take more registers than there are.
-static uint32_t paged_most_heads(uint32_t Dh, int kv_type) { return Dh == 512 && kv_type == G4A_KV_F32 ? 8 : 16; }
-
 struct g4a_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
@@ -918,7 +914,7 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
         for (int d = 0; d < 4; ++d) {
             snprintf(name, sizeof name, "g4a_paged_producer_d%d_%s", 64 << d, type);
             if (int rc = get_fn(ctx, &ctx->paged_producer[d][t], name)) return bail(rc);
-            for (int h = 0; h < (paged_most_heads(64u << d, t) == 16 ? 3 : 2); ++h) {
+            for (int h = 0; h < 3; ++h) {
                 for (int win = 0; win < 2; ++win) {
                     snprintf(name, sizeof name, "g4a_paged_decode%s_d%d_%s_h%d", win ? "_win" : "", 64 << d, type, 1 << h);
                     if (int rc = get_fn(ctx, &ctx->paged_decode[win][d][t][h], name)) return bail(rc);
@@ -2341,7 +2337,7 @@ constexpr uint32_t PAGED_FEW_UNITS = 8;
 constexpr uint32_t PAGED_UNITS = 2048;
 // Its workgroups per CU: [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
 constexpr uint32_t PAGED_WGS_PER_CU[4][2][3] = {
-    {{4, 3, 2}, {4, 2, 1}}, {{3, 2, 2}, {4, 2, 1}}, {{2, 2, 1}, {3, 2, 1}}, {{1, 1, 0}, {2, 1, 1}}};
+    {{4, 4, 2}, {4, 4, 4}}, {{3, 3, 2}, {4, 4, 3}}, {{2, 2, 1}, {3, 3, 2}}, {{1, 1, 1}, {1, 1, 1}}};
 
 // Index of a paged cache's head_dim among the kernels'.
 int paged_dh(uint32_t Dh) { return Dh == 64 ? 0 : Dh == 128 ? 1 : Dh == 256 ? 2 : 3; }
@@ -2473,7 +2469,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.room = uint32_t(room);
     p.span = a->sliding_window ? std::min(a->sliding_window, p.room) : p.room;
     p.group = a->Hq / cache->Hkv;
-    const int h = p.group <= 4 ? 0 : p.group <= 8 || paged_most_heads(cache->Dh, cache->kv_type) == 8 ? 1 : 2;
+    const int h = p.group <= 4 ? 0 : p.group <= 8 ? 1 : 2;
     const uint32_t heads = 4u << h;
     p.chunks = (p.group + heads - 1) / heads;
     p.units = cache->Hkv * p.chunks;

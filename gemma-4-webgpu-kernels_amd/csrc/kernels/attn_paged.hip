@@ -17,14 +17,18 @@
 //
 // A workgroup is 4 waves, each on every fourth tile of its part, with K and V of
 // the next tile in flight in registers (16-byte loads; no LDS in between):
-//   scores: K is the B operand of 16x16 MFMAs as it is loaded (lane = key l % 16 and
-//           a quarter of the dims), the query rows A, out of LDS: f32 pages on
+//   scores: K is the A operand of 16x16 MFMAs as it is loaded (lane = key l % 16 and a
+//           quarter of the dims), the query rows B, out of LDS: f32 pages on
 //           v_mfma_f32_16x16x4_f32, bf16 pages on v_mfma_f32_16x16x32_bf16 with the
-//           query as three bf16 parts, whose sum it is exactly;
-//   softmax: running maximum and sum in f32, a row of lanes per 4 heads;
-//   P.V:    v_mfma_f32_4x4x1_16b_f32, in f32: V is B as it is loaded (a lane's dims are
-//           columns of its block), P is A, one key of it broadcast to all blocks by the
-//           instruction; bf16 values become f32 by a shift.
+//           query as three bf16 parts, whose sum it is exactly. A lane then has four
+//           keys of one head;
+//   softmax: running maximum and sum in f32, across the four lanes of a head;
+//   P.V:    f32 pages on v_mfma_f32_4x4x1_16b_f32: V is B as it is loaded (a lane's dims
+//           are columns of its block), P is A, through LDS, one key of it broadcast to all
+//           blocks by the instruction. bf16 pages on v_mfma_f32_16x16x16_bf16: P is A as
+//           the softmax left it, in three bf16 parts, and a lane's four keys of a dim
+//           are B by two byte permutes of its loads. (4x4x1 takes 14 .. 16 cycles: 1.5
+//           of the 2.6 us a tile of 512 dims took from bf16 pages on it were its.)
 // The waves' partials join through LDS at the end.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -39,6 +43,9 @@
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// DPP: lane i of a row of 16 reads lane (i - 4 or 8) % 16.
+constexpr int ROW_ROR4 = 0x124, ROW_ROR8 = 0x128;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 template <int DH, typename KV, int NHQ>
@@ -46,22 +53,36 @@ struct PagedCfg {
     static constexpr bool BF = sizeof(KV) == 2;
     static constexpr int HR = 4 * NHQ;                       // query heads of a unit
     static constexpr int EL = 16 / (int)sizeof(KV);          // values of a 16-byte load
-    static constexpr int LG = DH / EL < 64 ? DH / EL : 64;   // lanes of a V row
-    static constexpr int LPK = DH / (EL * LG);               // V loads per row and lane
-    static constexpr int NK = 64 / LG;                       // V rows of a load
-    static constexpr int KI = 16 / NK;                       // V loads (times LPK) of a tile
-    static constexpr int CBSZ = KI == 16 ? 4 : KI == 8 ? 3 : KI == 4 ? 2 : 1;  // log2 KI: blocks a key of P goes to
-    static constexpr int NDG = EL * LPK;                     // 4 x 64 accumulators per 4 heads
     static constexpr int KC = DH / (4 * EL);                 // K loads of a tile
-    static constexpr int NM = NHQ == 1 ? 1 : NHQ == 2 ? 2 : 3;  // bf16: MFMAs per K load's dims
+    // f32 V: LG lanes of a row, LPK loads of a row and lane, NK rows of a load, KI * LPK loads of a tile
+    static constexpr int LG = DH / EL < 64 ? DH / EL : 64;
+    static constexpr int LPK = DH / (EL * LG);
+    static constexpr int NK = 64 / LG;
+    static constexpr int KI = 16 / NK;
+    static constexpr int CBSZ = KI == 16 ? 4 : KI == 8 ? 3 : KI == 4 ? 2 : 1;  // log2 KI: blocks a key of P goes to
+    // bf16 V: 16 lanes of EV dims of a row, four rows a lane, VB such blocks of dims
+    static constexpr int EV = DH / 16 < 8 ? DH / 16 : 8;
+    static constexpr int VB = DH / (16 * EV);
+    static constexpr int VW = BF ? EV / 2 : 4;               // words of a V load
+    static constexpr int VL = BF ? 4 * VB : KI * LPK;        // V loads of a tile
+    static constexpr int NM = NHQ == 1 ? 1 : NHQ == 2 ? 2 : 3;  // bf16: MFMAs for the three parts of 4 NHQ heads
+    // accumulators of a lane: f32 NHQ x EL LPK of 4 heads (a column a lane), bf16 VB EV of 16 rows
+    static constexpr int NA = BF ? VB * EV : NHQ * EL * LPK;
     // 16-byte query blocks in LDS: [K load][dim group][head], bf16 for each of three parts (half the
     // banks apart, as the lanes of one read take two of them)
     static constexpr int QPART = KC * 4 * HR + 8;
     static constexpr int QS = BF ? 3 * QPART : KC * 4 * HR;
     static constexpr int QL = (HR * DH / EL + 255) / 256;    // 16-byte (bf16: 32-byte) query pieces of a thread
-    static constexpr int ITEMS = NHQ * NDG * LG;             // = NHQ * DH: (4 heads, dim) of a partial
-    static constexpr int MRG = 4 * NHQ * NDG * 64;           // 16-byte blocks of the waves' accumulators
-    static constexpr int SM = (QS > MRG ? QS : MRG) * 16;    // the two never live at once
+    static constexpr int ITEMS = NHQ * DH;                   // (4 heads, dim) of a partial
+    static constexpr int ML = BF ? 16 * NHQ : 64;            // lanes that hand accumulators over
+    static constexpr int SM = (QS > 4 * NA * ML ? QS : 4 * NA * ML) * 16;  // queries and those never live at once
+    // Items in the accumulators' order: 4 heads hq, accumulator a, lane n of a row.
+    static constexpr int IL = BF ? 16 : LG, IA = DH / IL;
+    static __device__ __forceinline__ int hq(int item) { return item / DH; }
+    static __device__ __forceinline__ int dim(int item) {
+        const int n = item % IL, a = (item / IL) % IA;
+        return BF ? (a / EV) * 16 * EV + n * EV + a % EV : (a / EL) * LG * EL + n * EL + a % EL;
+    }
 };
 
 // A sequence's visible tiles: tokens [lo, len), tiles first .. first + n - 1 of 16 tokens.
@@ -105,48 +126,46 @@ __device__ __forceinline__ size_t uniform(size_t x) {
            (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
 }
 
-// N pieces of 16 bytes of a tile of K or V, PER of them `apart` bytes from one another in each
-// of N / PER rows that are `step` bytes apart; `off` is the lane's. Buffer loads: the row is a
-// scalar offset (as global loads each took a 64-bit vector sum, and registers for it), and what
-// lies behind the tile's `bytes` is not read. NT: past the caches.
-template <bool NT, int N, int PER, int APART>
-__device__ __forceinline__ void load_pieces(u32x4 (&x)[N], const char* tile, uint32_t bytes, uint32_t step, uint32_t off) {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(tile), 0, (int)bytes, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < N / PER; ++i)
-#pragma unroll
-        for (int y = 0; y < PER; ++y)
-            x[i * PER + y] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off + APART * y, (int)(i * step), NT ? 2 : 0);
+// A tile of K or V: `bytes` from its first row on, behind which nothing is read. Buffer loads:
+// a row is a scalar offset (as global loads each took a 64-bit vector sum, and registers for it).
+struct PagedTile {
+    __amdgpu_buffer_rsrc_t rsrc;
+};
+
+__device__ __forceinline__ PagedTile paged_tile(const void* pool, size_t at, uint32_t bytes) {
+    const char* const tile = reinterpret_cast<const char*>(pool) + uniform(at);
+    return {__builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(tile), 0, (int)bytes, 0x00020000)};
 }
 
-// One V row's element as f32.
-template <bool BF>
-__device__ __forceinline__ float v_value(const u32x4& v, int c) {
-    if constexpr (BF) return __uint_as_float(c & 1 ? v[c / 2] & 0xFFFF0000u : v[c / 2] << 16);
-    else return __uint_as_float(v[c]);
+// One load of 16 (or 8) bytes at the scalar offset `row` and the lane's `off`. NT: past the caches.
+template <bool NT, typename W>
+__device__ __forceinline__ void load_piece(W& x, const PagedTile& t, uint32_t row, uint32_t off) {
+    if constexpr (sizeof(W) == 16) x = __builtin_amdgcn_raw_buffer_load_b128(t.rsrc, (int)off, (int)row, NT ? 2 : 0);
+    else x = __builtin_amdgcn_raw_buffer_load_b64(t.rsrc, (int)off, (int)row, NT ? 2 : 0);
 }
 
-// acc[hq][dg] += P[key II of each block group][4 heads] x V's values of that load.
+// f32 pages: acc[hq][dims] += P[key II of each block group][4 heads] x V's values of that load.
 template <typename C, int II>
-__device__ __forceinline__ void pv_step(f4v (&acc)[C::HR / 4][C::NDG], const float (&pa)[C::HR / 4],
-                                        const u32x4 (&v)[C::KI * C::LPK]) {
+__device__ __forceinline__ void pv_step(f4v (&acc)[C::NA], const float (&pa)[C::HR / 4], const u32x4 (&v)[C::VL]) {
+    constexpr int ND = C::EL * C::LPK;
 #pragma unroll
     for (int e = 0; e < C::LPK; ++e)
 #pragma unroll
-        for (int c = 0; c < C::EL; ++c) {
-            const float b = v_value<C::BF>(v[II * C::LPK + e], c);
+        for (int c = 0; c < C::EL; ++c)
 #pragma unroll
             for (int hq = 0; hq < C::HR / 4; ++hq)
-                acc[hq][e * C::EL + c] =
-                    __builtin_amdgcn_mfma_f32_4x4x1f32(pa[hq], b, acc[hq][e * C::EL + c], C::CBSZ, II, 0);
-        }
+                acc[hq * ND + e * C::EL + c] = __builtin_amdgcn_mfma_f32_4x4x1f32(
+                    pa[hq], __uint_as_float(v[II * C::LPK + e][c]), acc[hq * ND + e * C::EL + c], C::CBSZ, II, 0);
 }
 
-template <typename C, int... II>
-__device__ __forceinline__ void pv_tile(f4v (&acc)[C::HR / 4][C::NDG], const float (&pa)[C::HR / 4],
-                                        const u32x4 (&v)[C::KI * C::LPK], std::integer_sequence<int, II...>) {
-    (pv_step<C, II>(acc, pa, v), ...);
+template <typename C, typename After, int... II>
+__device__ __forceinline__ void pv_tile(f4v (&acc)[C::NA], const float (&pa)[C::HR / 4], const u32x4 (&v)[C::VL],
+                                        const After& after, std::integer_sequence<int, II...>) {
+    ((pv_step<C, II>(acc, pa, v), after(II)), ...);
 }
+
+typedef short bf4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4v __attribute__((ext_vector_type(4)));
 
 // WIN: a window's rows, which stay in the caches until the next step; a whole context's K and V
 // are read past them (16 ragged sequences 58.0 -> 55.3 us, eight of up to 131072 keys 163 -> 156;
@@ -155,10 +174,10 @@ template <int DH, typename KV, int NHQ, bool WIN>
 __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     using C = PagedCfg<DH, KV, NHQ>;
     constexpr bool BF = C::BF;
-    constexpr int HR = C::HR, EL = C::EL, LG = C::LG, LPK = C::LPK, KI = C::KI, NDG = C::NDG, KC = C::KC, NM = C::NM,
-                  QL = C::QL;
+    constexpr int HR = C::HR, EL = C::EL, KC = C::KC, NM = C::NM, NA = C::NA, QL = C::QL;
+    using VWord = uint32_t __attribute__((ext_vector_type(C::VW)));
     __shared__ __attribute__((aligned(16))) char smem[C::SM];
-    __shared__ __attribute__((aligned(16))) float p_s[4][NHQ * 64];
+    __shared__ __attribute__((aligned(16))) float p_s[4][BF ? 4 : NHQ * 64];
     __shared__ __attribute__((aligned(16))) float f_s[4][HR];
     __shared__ float m_s[4][HR], l_s[4][HR];
     u32x4* const qs = reinterpret_cast<u32x4*>(smem);
@@ -225,7 +244,10 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     const uint32_t nh = min((uint32_t)HR, p.group - (j - kvh * p.chunks) * HR);
 
     const uint32_t row_bytes = c.Hkv * DH * sizeof(KV);  // (at most 2 MiB)
-    const uint32_t koff = key * row_bytes + 16 * g4, voff = (lane / LG) * KI * row_bytes + 16 * (lane % LG);
+    // K: lane (g4, key) its key's dims; V: f32 lane LG r + n row KI r, bf16 lane (g4, n) row 4 g4
+    const uint32_t koff = key * row_bytes + 16 * g4;
+    const uint32_t voff = BF ? 4 * g4 * row_bytes + 4 * C::VW * key
+                             : (lane / C::LG) * C::KI * row_bytes + 16 * (lane % C::LG);
 
     auto page_of = [&](uint32_t t) {
         const uint32_t no = (sp.first + t) >> (c.page_shift - 4);
@@ -235,14 +257,22 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
         const uint32_t r = ((sp.first + t) * 16) & ((1u << c.page_shift) - 1);
         return ((size_t)(page < c.n_pages ? page : 0u) * c.page_stride + ((size_t)r * c.Hkv + kvh) * DH) * sizeof(KV);
     };
-    u32x4 k[KC], v[KI * LPK];
+    // 16 heads at 512 dims: K and V take turns in one set of registers, V's pieces loaded where K's have
+    // been used and K's next where V's have, as there is no room for both. (With 8 heads, and two workgroups
+    // a CU for it, eight sequences of up to 131072 keys took 146 us, 133 with both in flight.)
+    constexpr bool TURNS = DH == 512 && NHQ == 4;
+    VWord v[C::VL];  // bf16: [row][block of dims]
+    u32x4 k_own[TURNS ? 1 : KC];
+    u32x4 (&k)[KC] = [&]() -> u32x4 (&)[KC] {
+        if constexpr (TURNS) return v;
+        else return k_own;
+    }();
+    static_assert(C::VL % KC == 0 && (!TURNS || KC == C::VL), "pieces of V for each of K");
     const uint32_t tile_bytes = 16 * row_bytes;
-    auto load_k = [&](size_t at) {
-        load_pieces<!WIN, KC, KC, 64>(k, reinterpret_cast<const char*>(c.k) + uniform(at), tile_bytes, 0, koff);
-    };
-    auto load_v = [&](size_t at) {
-        load_pieces<!WIN, KI * LPK, LPK, 1024>(v, reinterpret_cast<const char*>(c.v) + uniform(at), tile_bytes, row_bytes,
-                                               voff);
+    auto load_k = [&](const PagedTile& t, int i) { load_piece<!WIN>(k[i], t, 0, koff + 64 * i); };
+    auto load_v = [&](const PagedTile& t, int i) {  // bf16: row i / VB, block i % VB; f32: rows i / LPK
+        constexpr int PER = BF ? C::VB : C::LPK;
+        load_piece<!WIN>(v[i], t, i / PER * row_bytes, voff + i % PER * (BF ? 256 : 1024));
     };
     // ---- the query rows into LDS, EL dims of a head a piece; their loads go out first ----
     f4v qr[QL][EL / 4];
@@ -262,8 +292,9 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     uint32_t page = page_of(min(t, e - 1)), page_next = t + 4 < e ? page_of(t + 4) : 0u;
     {
         const size_t off = tile_at(page, min(t, e - 1));
-        load_k(off);
-        load_v(off);
+        const PagedTile kt = paged_tile(c.k, off, tile_bytes);
+#pragma unroll
+        for (int i = 0; i < KC; ++i) load_k(kt, i);
     }
 #pragma unroll
     for (int i = 0; i < QL; ++i) {
@@ -287,7 +318,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
             qs[x] = __builtin_bit_cast(u32x4, qr[i][0]);
         }
     }
-    // bf16: this lane's query block of the first K load in each MFMA: rows of 4 * NHQ heads, the parts in order
+    // bf16: this lane's query block of the first K load in each MFMA: columns of 4 * NHQ heads, the parts in order
     // (NHQ 1: the fourth repeats the third, and is not summed; NHQ 2: so does the second MFMA's second half)
     int qi[NM];
 #pragma unroll
@@ -298,21 +329,33 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
 
     barrier_lds();  // (K and V stay in flight across it)
 
-    // lane (g4, key): heads 4 * (g4 % NHQ) + r of the tile's key
-    float m[4], l[4];
-    f4v acc[NHQ][NDG];
+    // lane (g4, n): keys 4 g4 + r of the tile, head n % HR of the unit (all of n's repeats alike)
+    float m = G4A_NEG_INF, l = 0.0f;
+    f4v acc[NA];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) m[r] = G4A_NEG_INF, l[r] = 0.0f;
-#pragma unroll
-    for (int hq = 0; hq < NHQ; ++hq)
-#pragma unroll
-        for (int d = 0; d < NDG; ++d) acc[hq][d] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int d = 0; d < NA; ++d) acc[d] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // one tile; MORE: with the loads of the wave's next
-    auto tile = [&](auto last) {
-        constexpr bool MORE = !decltype(last)::value;
+    // One tile; MORE: a piece of the wave's next is loaded where this one's has been used; FIRST: V is
+    // loaded between the scores' MFMAs, as ahead of them its loads held up the first of them. (The empty
+    // scheduling barriers keep the reads of all query rows, and V's permutes, from being gathered ahead of
+    // the first MFMA, in more registers than there are.)
+    auto tile = [&](auto first, auto more) {
+        constexpr bool FIRST = decltype(first)::value || TURNS, MORE = decltype(more)::value;
         const uint32_t page_after = MORE && t + 8 < e ? page_of(t + 8) : 0u;
-        const size_t off = MORE ? tile_at(page_next, t + 4) : 0;
+        const size_t next = MORE ? tile_at(page_next, t + 4) : 0;
+        const PagedTile kt = paged_tile(c.k, next, tile_bytes);
+        const PagedTile vt = paged_tile(c.v, next, tile_bytes), vt0 = paged_tile(c.v, FIRST ? tile_at(page, t) : 0, tile_bytes);
+        auto after_k = [&](int i) {
+            if constexpr (FIRST)
+#pragma unroll
+                for (int x = i * C::VL / KC; x < (i + 1) * C::VL / KC; ++x) load_v(vt0, x);
+            if constexpr (!TURNS && MORE) load_k(kt, i);
+        };
+        auto after_v = [&](int i) {
+            if constexpr (!MORE) return;
+            else if constexpr (TURNS) load_k(kt, i);
+            else load_v(vt, i);
+        };
         // scores
         float x[4];
         if constexpr (BF) {
@@ -320,23 +363,24 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
 #pragma unroll
             for (int y = 0; y < NM; ++y) d[y] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < KC; ++i)
+            for (int i = 0; i < KC; ++i) {
 #pragma unroll
                 for (int y = 0; y < NM; ++y)
                     d[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, qs[qi[y] + i * 4 * HR]), __builtin_bit_cast(bf16x8, k[i]), d[y], 0, 0,
+                        __builtin_bit_cast(bf16x8, k[i]), __builtin_bit_cast(bf16x8, qs[qi[y] + i * 4 * HR]), d[y], 0, 0,
                         0);
+                after_k(i);
+                if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < 4; ++r) {  // the parts of a head are in columns HR apart
                 if constexpr (NHQ == 4) {
                     x[r] = (d[2][r] + d[1][r]) + d[0][r];
                 } else if constexpr (NHQ == 2) {
-                    const float2 y = g4a_pair32(d[0][r]);  // the first and second parts
-                    x[r] = (d[1][r] + y.y) + y.x;
+                    x[r] = d[1][r] + (d[0][r] + g4a_dpp<ROW_ROR8>(d[0][r]));
                 } else {
-                    const float2 y = g4a_pair16(d[0][r]);  // lanes 0 .. 31: first and second part, others: the third
-                    const float2 z = g4a_pair32(y.x + (g4 < 2 ? y.y : 0.0f));
-                    x[r] = z.x + z.y;
+                    const float y = key < 12 ? d[0][r] : 0.0f, z = y + g4a_dpp<ROW_ROR8>(y);
+                    x[r] = z + g4a_dpp<ROW_ROR4>(z);
                 }
             }
         } else {
@@ -348,80 +392,140 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
                 const u32x4 qa = qs[(i * 4 + g4) * HR + key % HR];
 #pragma unroll
                 for (int y = 0; y < 4; ++y)
-                    d[y] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(qa[y]), __uint_as_float(k[i][y]), d[y],
-                                                                0, 0, 0);
+                    d[y] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i][y]), __uint_as_float(qa[y]), d[y], 0, 0,
+                                                                0);
+                after_k(i);
+                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = (d[0][r] + d[1][r]) + (d[2][r] + d[3][r]);
         }
-        if constexpr (MORE) load_k(off);
 
         // running maximum and sum
         const uint32_t t0 = (sp.first + t) * 16;
         const bool hidden = page >= c.n_pages;
         const uint32_t lo = sp.lo > t0 ? sp.lo - t0 : 0u, hi = hidden ? 0u : min(16u, sp.len - t0);
-        const bool seen = (uint32_t)key >= lo && (uint32_t)key < hi;
-        float corr[4];
-        bool moved = false;
         f4v pr;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             float y = x[r] * p.scale;
             if (p.softcap > 0.0f) y = p.softcap * tanhf(y / p.softcap);
-            y = seen ? y : G4A_NEG_INF;
-            const float mn = fmaxf(m[r], g4a_row_max16(y));
-            corr[r] = m[r] == G4A_NEG_INF ? 0.0f : expf(m[r] - mn);
-            pr[r] = y == G4A_NEG_INF ? 0.0f : expf(y - mn);
-            moved |= mn != m[r];
-            l[r] = l[r] * corr[r] + pr[r];
-            m[r] = mn;
+            const uint32_t row = 4 * g4 + r;
+            pr[r] = row >= lo && row < hi ? y : G4A_NEG_INF;
         }
-        // P to lane 4 * key + head, the A operand of 4x4x1
-        if (g4 < NHQ) *reinterpret_cast<f4v*>(&p_s[w][4 * (16 * g4 + key)]) = pr;
+        const float mn = fmaxf(m, g4a_col_max4(fmaxf(fmaxf(pr[0], pr[1]), fmaxf(pr[2], pr[3]))));
+        const float corr = m == G4A_NEG_INF ? 0.0f : expf(m - mn);
+        const bool moved = mn != m;
+        m = mn;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pr[r] = pr[r] == G4A_NEG_INF ? 0.0f : expf(pr[r] - mn);
+        l = l * corr + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
         if (__ballot(moved)) {
 #pragma unroll
-            for (int hq = 0; hq < NHQ; ++hq)
+            for (int hq = 0; hq < (BF ? 1 : NHQ); ++hq)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float f = g4a_lane(corr[r], 16 * hq);
+                for (int r = 0; r < 4; ++r) {  // the lanes of a head hold its factor
+                    const float f = BF && NHQ > 1 ? __shfl(corr, 4 * (g4 % NHQ) + r) : g4a_lane(corr, 4 * hq + r);
 #pragma unroll
-                    for (int d = 0; d < NDG; ++d) acc[hq][d][r] *= f;
+                    for (int d = 0; d < (BF ? NA : NA / NHQ); ++d) acc[hq * (NA / NHQ) + d][r] *= f;
                 }
         }
-        __builtin_amdgcn_wave_barrier();
-        float pa[NHQ];
-#pragma unroll
-        for (int hq = 0; hq < NHQ; ++hq) pa[hq] = p_s[w][64 * hq + lane];
-        __builtin_amdgcn_wave_barrier();
         // what no token was written to may hold anything, and 0 times it is not 0
         if (lo > 0 || hi < 16) {
 #pragma unroll
-            for (int i = 0; i < KI; ++i) {
-                const uint32_t row = i + KI * (lane / LG);
-                const uint32_t keep = row >= lo && row < hi ? 0xFFFFFFFFu : 0u;
-#pragma unroll
-                for (int y = 0; y < LPK; ++y) v[i * LPK + y] &= keep;
+            for (int i = 0; i < C::VL; ++i) {
+                const uint32_t row = BF ? 4 * g4 + i / C::VB : i / C::LPK + C::KI * (lane / C::LG);
+                v[i] &= row >= lo && row < hi ? 0xFFFFFFFFu : 0u;
             }
         }
-        pv_tile<C>(acc, pa, v, std::make_integer_sequence<int, KI>());
-        if constexpr (MORE) load_v(off);
+        if constexpr (BF) {
+            // P's rows as the query's columns: part by part, a head's parts HR rows apart
+            bf4 pa[NM];
+            bf16x4v part[3];
+            f4v rest = pr;
+#pragma unroll
+            for (int y = 0; y < 3; ++y) {
+                part[y] = __builtin_convertvector(rest, bf16x4v);
+                rest -= __builtin_convertvector(part[y], f4v);
+            }
+            const bf4 zero = {0, 0, 0, 0};
+            if constexpr (NHQ == 4) {
+#pragma unroll
+                for (int y = 0; y < 3; ++y) pa[y] = __builtin_bit_cast(bf4, part[y]);
+            } else if constexpr (NHQ == 2) {
+                pa[0] = key < 8 ? __builtin_bit_cast(bf4, part[0]) : __builtin_bit_cast(bf4, part[1]);
+                pa[1] = key < 8 ? __builtin_bit_cast(bf4, part[2]) : zero;
+            } else {
+                pa[0] = key < 4    ? __builtin_bit_cast(bf4, part[0])
+                        : key < 8  ? __builtin_bit_cast(bf4, part[1])
+                        : key < 12 ? __builtin_bit_cast(bf4, part[2])
+                                   : zero;
+            }
+#pragma unroll
+            for (int y = 0; y < C::VB; ++y) {
+#pragma unroll
+                for (int e = 0; e < C::EV; ++e) {
+                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;  // rows i, i + 1 of a dim into a word
+                    const uint32_t b0 = __builtin_amdgcn_perm(v[C::VB + y][e / 2], v[y][e / 2], sel);
+                    const uint32_t b1 = __builtin_amdgcn_perm(v[3 * C::VB + y][e / 2], v[2 * C::VB + y][e / 2], sel);
+                    const bf4 b = __builtin_bit_cast(bf4, (uint64_t)b1 << 32 | b0);
+#pragma unroll
+                    for (int z = 0; z < NM; ++z)
+                        acc[y * C::EV + e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pa[z], b, acc[y * C::EV + e], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) after_v(i * C::VB + y);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            // P to lane 4 * key + head, the A operand of 4x4x1
+            if (key < HR) *reinterpret_cast<f4v*>(&p_s[w][16 * key + 4 * g4]) = pr;
+            __builtin_amdgcn_wave_barrier();
+            float pa[NHQ];
+#pragma unroll
+            for (int hq = 0; hq < NHQ; ++hq) pa[hq] = p_s[w][16 * (4 * hq + (lane & 3)) + (lane >> 2)];
+            __builtin_amdgcn_wave_barrier();
+            auto reload = [&](int ii) {
+#pragma unroll
+                for (int x = 0; x < C::LPK; ++x) after_v(ii * C::LPK + x);
+            };
+            pv_tile<C>(acc, pa, v, reload, std::make_integer_sequence<int, C::KI>());
+        }
         page = page_next;
         page_next = page_after;
     };
-    for (; t + 4 < e; t += 4) tile(std::false_type());
-    if (t < e) tile(std::true_type());
+    const std::true_type yes;
+    const std::false_type no;
+    if constexpr (TURNS) {
+        for (; t + 4 < e; t += 4) tile(yes, yes);
+        if (t < e) tile(yes, no);
+    } else if (t + 4 < e) {
+        tile(yes, yes);
+        for (t += 4; t + 4 < e; t += 4) tile(no, yes);
+        tile(no, no);
+    } else if (t < e) {
+        tile(yes, no);
+    }
 
     // ---- the waves' partials, through LDS ----
-#pragma unroll
-    for (int r = 0; r < 4; ++r) l[r] = g4a_row_sum16(l[r]);
-    if (key == 0 && g4 < NHQ)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) m_s[w][4 * g4 + r] = m[r], l_s[w][4 * g4 + r] = l[r];
+    l = g4a_col_sum4(l);
+    if (lane < HR) m_s[w][lane] = m, l_s[w][lane] = l;
     barrier_lds();  // every wave is done with the query rows, where the accumulators go
 #pragma unroll
-    for (int hq = 0; hq < NHQ; ++hq)
+    for (int d = 0; d < NA; ++d) {
+        if constexpr (BF && NHQ < 4) {  // the rows of a head's parts, in lanes 16 NHQ apart
 #pragma unroll
-        for (int d = 0; d < NDG; ++d) mrg[((w * NHQ + hq) * NDG + d) * 64 + lane] = acc[hq][d];
+            for (int r = 0; r < 4; ++r) {
+                float2 y = g4a_pair32(acc[d][r]);
+                acc[d][r] = y.x + y.y;
+                if constexpr (NHQ == 1) {
+                    y = g4a_pair16(acc[d][r]);
+                    acc[d][r] = y.x + y.y;
+                }
+            }
+        }
+        if (C::ML == 64 || lane < C::ML) mrg[(w * NA + d) * C::ML + lane] = acc[d];
+    }
     const bool whole = parts == 1;
     if (tid < HR) {
         float M = G4A_NEG_INF, L = 0.0f, f[4];
@@ -444,18 +548,22 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     barrier_lds();
     f4v* const dst = reinterpret_cast<f4v*>(p.part) + (size_t)at * C::ITEMS;
     for (int i = tid; i < C::ITEMS; i += 256) {
-        const int hq = i / (NDG * LG), d = (i / LG) % NDG, lg = i % LG;
+        const int hq = C::hq(i), n = i % C::IL, a = (i / C::IL) % C::IA;
         f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
             const f4v f = *reinterpret_cast<const f4v*>(&f_s[y][4 * hq]);
-            f4v a = mrg[((y * NHQ + hq) * NDG + d) * 64 + lg];
+            if constexpr (BF) {
+                o += mrg[(y * NA + a) * C::ML + 16 * hq + n] * f;
+            } else {
+                f4v x = mrg[(y * NA + hq * C::IA + a) * 64 + n];
 #pragma unroll
-            for (int z = 1; z < C::NK; ++z) a += mrg[((y * NHQ + hq) * NDG + d) * 64 + z * LG + lg];
-            o += a * f;
+                for (int z = 1; z < C::NK; ++z) x += mrg[(y * NA + hq * C::IA + a) * 64 + z * C::LG + n];
+                o += x * f;
+            }
         }
         if (whole) {
-            const int dim = (d / EL) * LG * EL + lg * EL + d % EL;
+            const int dim = C::dim(i);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (4 * hq + r < (int)nh) p.out[((size_t)b * p.Hq + h0 + 4 * hq + r) * DH + dim] = o[r];
@@ -486,9 +594,8 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
     const int tid = threadIdx.x, it = tid % CI, gr = tid / CI;
     const uint32_t item = blockIdx.x % (C::ITEMS / CI) * CI + it;
     // (the block's items are of one group of 4 heads)
-    const int hq = item / (C::NDG * C::LG), d = (item / C::LG) % C::NDG, lg = item % C::LG;
-    const int dim = (d / C::EL) * C::LG * C::EL + lg * C::EL + d % C::EL;
-    static_assert(C::NDG * C::LG % CI == 0, "a block's items share their heads");
+    const int hq = C::hq(item), dim = C::dim(item);
+    static_assert(DH % CI == 0, "a block's items share their heads");
     const uint32_t quota = load_scalar(p.offs, 0), off = load_scalar(p.offs, 1 + b);
     const PagedSpan sp = paged_span(p, load_scalar(p.c.len, b));
     f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -567,10 +674,9 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
     G4A_PAGED_DECODE(dh, f32, float, nhq, occ_f32)         \
     G4A_PAGED_DECODE(dh, bf16, __bf16, nhq, occ_bf16)
 // The second bound: workgroups of a CU, as the registers (and LDS) leave room for.
-G4A_PAGED_DECODE_TYPES(64, 1, 4, 4) G4A_PAGED_DECODE_TYPES(64, 2, 3, 2) G4A_PAGED_DECODE_TYPES(64, 4, 2, 1)
-G4A_PAGED_DECODE_TYPES(128, 1, 3, 4) G4A_PAGED_DECODE_TYPES(128, 2, 2, 2) G4A_PAGED_DECODE_TYPES(128, 4, 2, 1)
-G4A_PAGED_DECODE_TYPES(256, 1, 2, 3) G4A_PAGED_DECODE_TYPES(256, 2, 2, 2) G4A_PAGED_DECODE_TYPES(256, 4, 1, 1)
-G4A_PAGED_DECODE_TYPES(512, 1, 1, 2) G4A_PAGED_DECODE_TYPES(512, 2, 1, 1)
-G4A_PAGED_DECODE(512, bf16, __bf16, 4, 1)  // (f32: two units of 8 heads, 16 have too many registers)
+G4A_PAGED_DECODE_TYPES(64, 1, 4, 4) G4A_PAGED_DECODE_TYPES(64, 2, 4, 4) G4A_PAGED_DECODE_TYPES(64, 4, 2, 4)
+G4A_PAGED_DECODE_TYPES(128, 1, 3, 4) G4A_PAGED_DECODE_TYPES(128, 2, 3, 4) G4A_PAGED_DECODE_TYPES(128, 4, 2, 3)
+G4A_PAGED_DECODE_TYPES(256, 1, 2, 3) G4A_PAGED_DECODE_TYPES(256, 2, 2, 3) G4A_PAGED_DECODE_TYPES(256, 4, 1, 2)
+G4A_PAGED_DECODE_TYPES(512, 1, 1, 1) G4A_PAGED_DECODE_TYPES(512, 2, 1, 1) G4A_PAGED_DECODE_TYPES(512, 4, 1, 1)
 #undef G4A_PAGED_DECODE_TYPES
 #undef G4A_PAGED_DECODE
