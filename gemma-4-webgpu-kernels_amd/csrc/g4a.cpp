@@ -2331,6 +2331,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 constexpr uint32_t PAGED_MIN_PART = 4;
 // Most parts of a unit: the merge keeps a weight for each (attn_paged.hip).
 constexpr uint32_t PAGED_MAX_PARTS = 1024;
+// Most sequences of a launch (attn_paged.hip).
+constexpr uint32_t PAGED_SEQS = 1024;
 // Units up to which a merge block takes 16 items of one, not 64.
 constexpr uint32_t PAGED_FEW_UNITS = 8;
 // Most units of a launch (but for a sequence that has more).
@@ -2482,8 +2484,9 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.softcap = a->attn_softcap;
     const int d = paged_dh(cache->Dh), t = int(cache->kv_type);
     const uint32_t resident = uint32_t(std::max(ctx->cu_count, 1)) * PAGED_WGS_PER_CU[d][t][h];
-    // launches of at most PAGED_UNITS units, which bounds the partials' memory
-    const uint32_t most = std::min(cache->n_seqs, std::max(1u, PAGED_UNITS / p.units));
+    // launches of at most PAGED_UNITS units, which bounds the partials' memory, and of as many sequences as
+    // the kernel counts
+    const uint32_t most = std::min({cache->n_seqs, std::max(1u, PAGED_UNITS / p.units), PAGED_SEQS});
     // parts: as many as the GPU runs at once, no more of units that leave room for a few parts each, and else
     // about as many again; none of fewer tiles than there are
     auto shares = [&](uint32_t seqs, uint32_t* spread, uint32_t* fit) {
@@ -2512,8 +2515,8 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
                             "paged decode", true))
             return rc;
         const uint32_t wide = units > PAGED_FEW_UNITS, blocks = uint32_t(item / 4) / (wide ? 64 : 16);
-        if (int rc = launch(ctx, ctx->paged_combine[wide][d][t][h], dim3(blocks * units, 1, 1), dim3(256, 1, 1), p,
-                            "paged combine", true))
+        if (int rc = launch(ctx, ctx->paged_combine[wide][d][t][h], dim3(blocks * units, 1, 1),
+                            dim3(wide ? 256 : 1024, 1, 1), p, "paged combine", true))
             return rc;
     }
     return G4A_OK;

@@ -75,7 +75,9 @@ struct PagedCfg {
     static constexpr int QL = (HR * DH / EL + 255) / 256;    // 16-byte (bf16: 32-byte) query pieces of a thread
     static constexpr int ITEMS = NHQ * DH;                   // (4 heads, dim) of a partial
     static constexpr int ML = BF ? 16 * NHQ : 64;            // lanes that hand accumulators over
-    static constexpr int SM = (QS > 4 * NA * ML ? QS : 4 * NA * ML) * 16;  // queries and those never live at once
+    // queries, those and the sequences' lengths never live at once
+    static constexpr int SM = (QS > 4 * NA * ML ? QS : 4 * NA * ML) * 16;
+    static_assert(SM >= 4096, "the lengths of PAGED_SEQS sequences");
     // Items in the accumulators' order: 4 heads hq, accumulator a, lane n of a row.
     static constexpr int IL = BF ? 16 : LG, IA = DH / IL;
     static __device__ __forceinline__ int hq(int item) { return item / DH; }
@@ -84,6 +86,8 @@ struct PagedCfg {
         return BF ? (a / EV) * 16 * EV + n * EV + a % EV : (a / EL) * LG * EL + n * EL + a % EL;
     }
 };
+
+constexpr uint32_t PAGED_SEQS = 1024;  // of a launch, at most
 
 // A sequence's visible tiles: tokens [lo, len), tiles first .. first + n - 1 of 16 tokens.
 struct PagedSpan {
@@ -97,6 +101,14 @@ __device__ __forceinline__ PagedSpan paged_span(const G4aPagedAttnParams& p, uin
     s.first = s.lo / 16;
     s.n = s.len ? (s.len - 1) / 16 + 1 - s.first : 0u;
     return s;
+}
+
+// ceil(tiles / quota) parts of a unit, by a reciprocal that is rounded down by 2^-20: exact below
+// 2^19 tiles, never more. (An integer division each took 2 us of a call of 128 sequences. Every
+// workgroup and the merge compute the same.)
+__device__ __forceinline__ uint32_t paged_parts(uint32_t tiles, uint32_t quota) {
+    const float inv = __builtin_amdgcn_rcpf((float)quota) * (1.0f - 0x1p-20f);
+    return tiles ? 1u + (uint32_t)(((float)tiles - 0.5f) * inv) : 0u;
 }
 
 // Sums over the lanes up to and with this one: four shifts within the rows of 16 lanes,
@@ -189,14 +201,19 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     // ---- this workgroup's part: every wave sums the lengths, a span of `each` sequences a lane ----
     const uint32_t n = c.n_seqs, each = (n + 63) / 64;
     const uint32_t my_len = lane < (int)n && each == 1 ? c.len[lane] : 0u;
-    auto lane_tiles = [&](uint32_t b) { return b < n ? paged_span(p, each == 1 ? my_len : c.len[b]).n : 0u; };
+    // (more than one a lane: through LDS, by every wave alike. Short loops: sixteen lengths a lane in registers,
+    // unrolled, took 1.6 us more of a small call, in code that no cache holds yet.)
+    uint32_t* const lens = reinterpret_cast<uint32_t*>(smem);
+    if (each > 1)
+        for (uint32_t b = lane; b < n; b += 64) lens[b] = c.len[b];
+    auto lane_tiles = [&](uint32_t b) { return b < n ? paged_span(p, each == 1 ? my_len : lens[b]).n : 0u; };
     uint32_t mine = 0;
     for (uint32_t i = 0; i < each; ++i) mine += lane_tiles(lane * each + i);
     const uint32_t total = (uint32_t)__builtin_amdgcn_readlane(wave_incl_sum(mine), 63) * p.units;
     uint32_t quota = max((total + p.spread - 1) / p.spread, p.min_part), upto;
     if (quota < 2 * p.min_part) quota = (quota + p.min_part - 1) / p.min_part * p.min_part;  // (whole rounds of the waves)
     // parts of a sequence's units; the first few quotas may give more parts than `fit` holds, the last cannot
-    auto parts_of = [&](uint32_t tiles) { return p.units * ((tiles + quota - 1) / quota); };
+    auto parts_of = [&](uint32_t tiles) { return p.units * paged_parts(tiles, quota); };
     for (int tries = 0;; ++tries) {
         mine = 0;
         for (uint32_t i = 0; i < each; ++i) mine += parts_of(lane_tiles(lane * each + i));
@@ -234,10 +251,11 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
             }
             base += __builtin_amdgcn_readlane(u, 63);
         }
-        len = load_scalar(c.len, b);
+        len = __builtin_amdgcn_readfirstlane(lens[b]);
+        barrier_lds();  // every wave has read the lengths: the query rows go there
     }
     const PagedSpan sp = paged_span(p, len);
-    const uint32_t parts = (sp.n + quota - 1) / quota, j = (at - base) / parts, part = at - base - j * parts;
+    const uint32_t parts = __builtin_amdgcn_readfirstlane(paged_parts(sp.n, quota)), j = (at - base) / parts, part = at - base - j * parts;
     const uint32_t floor = sp.n / parts, more = sp.n % parts;
     const uint32_t s = part * floor + min(part, more), e = s + floor + (part < more ? 1u : 0u);  // its tiles
     const uint32_t kvh = j / p.chunks, h0 = kvh * p.group + (j - kvh * p.chunks) * HR;
@@ -574,20 +592,23 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
 }
 
 // Merges the partials of units that more than one workgroup worked on, and writes the
-// zeros of sequences without tokens. A block takes CI items (4 heads, one dim) of a
-// unit, 256 / CI groups of threads every such part of it: CI 16 where there are few
-// units of many parts, 64 where there are many units. A thread's first partial is
-// loaded with the parts' maxima and sums, ahead of the weights e^(m - M), which are
-// computed a part a thread and meet in LDS.
+// zeros of sequences without tokens. A block of W waves takes CI items (4 heads, one
+// dim) of a unit, 64 W / CI groups of threads every such part of it: 16 items and 16
+// waves where there are few units of many parts (256 parts of 512 dims: 16 loads a
+// thread on 4 waves took 6.5 us, half of them waiting in turn), 64 items and 4 waves
+// where there are many units. A thread's first partial is loaded with the parts' maxima
+// and sums, ahead of the weights e^(m - M), which are computed a part a thread and meet
+// in LDS.
 constexpr int PAGED_PARTS = 1024;  // of a unit, at most
 
-template <int DH, typename KV, int NHQ, int CI>
+template <int DH, typename KV, int NHQ, int CI, int W>
 __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
     using C = PagedCfg<DH, KV, NHQ>;
-    constexpr int CG = 256 / CI;
+    constexpr int NT = 64 * W, CG = NT / CI;
+    static_assert(CI == 16 || CI == 64, "a wave's groups meet by columns of 16 lanes");
     __shared__ f4v w_s[PAGED_PARTS];
-    __shared__ f4v o_s[CG][CI];
-    __shared__ f4v r_s[2][4];
+    __shared__ f4v o_s[W][CI];
+    __shared__ f4v r_s[2][W];
     const uint32_t u = blockIdx.x / (C::ITEMS / CI), b = u / p.units, j = u - b * p.units;
     const uint32_t kvh = j / p.chunks, hc = j - kvh * p.chunks;
     const uint32_t h0 = kvh * p.group + hc * C::HR, nh = min((uint32_t)C::HR, p.group - hc * C::HR);
@@ -600,7 +621,7 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
     const PagedSpan sp = paged_span(p, load_scalar(p.c.len, b));
     f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
     if (sp.n) {
-        const uint32_t parts = (sp.n + quota - 1) / quota, slot0 = off + j * parts;
+        const uint32_t parts = __builtin_amdgcn_readfirstlane(paged_parts(sp.n, quota)), slot0 = off + j * parts;
         if (parts == 1) return;
         const f4v* const part = reinterpret_cast<const f4v*>(p.part) + (size_t)slot0 * C::ITEMS + item;
         const f4v* const ml = reinterpret_cast<const f4v*>(p.part_ml) + (size_t)slot0 * 2 * NHQ + hq;
@@ -609,11 +630,11 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
         const f4v m0 = has ? ml[(size_t)tid * 2 * NHQ] : none, l0 = has ? ml[(size_t)tid * 2 * NHQ + NHQ] : f4v{};
         const f4v o0 = gr < (int)parts ? part[(size_t)gr * C::ITEMS] : f4v{};
         f4v M = m0;
-        for (uint32_t i = tid + 256; i < parts; i += 256)
+        for (uint32_t i = tid + NT; i < parts; i += NT)
 #pragma unroll
             for (int r = 0; r < 4; ++r) M[r] = fmaxf(M[r], ml[(size_t)i * 2 * NHQ][r]);
-        // (parts of the first waves only, but for more than 256)
-        const int waves = parts >= 256 ? 4 : (int)(parts + 63) / 64, wave = tid / 64;
+        // (parts of the first waves only, but for more than NT)
+        const int waves = parts >= NT ? W : (int)(parts + 63) / 64, wave = tid / 64;
         if (wave < waves) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) M[r] = g4a_wave_max(M[r]);
@@ -628,8 +649,8 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
         }
         f4v L = {0.0f, 0.0f, 0.0f, 0.0f};
         if (wave < waves) {
-            for (uint32_t i = tid; i < parts; i += 256) {
-                const f4v m = i < 256 ? m0 : ml[(size_t)i * 2 * NHQ], l = i < 256 ? l0 : ml[(size_t)i * 2 * NHQ + NHQ];
+            for (uint32_t i = tid; i < parts; i += NT) {
+                const f4v m = i < NT ? m0 : ml[(size_t)i * 2 * NHQ], l = i < NT ? l0 : ml[(size_t)i * 2 * NHQ + NHQ];
                 f4v f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) f[r] = m[r] == G4A_NEG_INF ? 0.0f : expf(m[r] - M[r]);
@@ -644,12 +665,16 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
         if (gr < (int)parts) o = o0 * w_s[gr];
 #pragma unroll 4
         for (uint32_t i = gr + CG; i < parts; i += CG) o += part[(size_t)i * C::ITEMS] * w_s[i];
-        o_s[gr][it] = o;
+        if constexpr (CI == 16)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = g4a_col_sum4(o[r]);
+        if (tid % 64 < CI) o_s[wave][it] = o;
         __syncthreads();
         if (gr) return;
         L = r_s[1][0];
         for (int i = 1; i < waves; ++i) L += r_s[1][i];
-        for (int i = 1; i < min(CG, (int)parts); ++i) o += o_s[i][it];
+#pragma unroll
+        for (int i = 1; i < W; ++i) o += o_s[i][it];
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = L[r] != 0.0f ? o[r] / L[r] : 0.0f;
     }
@@ -666,10 +691,10 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
         G4aPagedAttnParams p) { paged_decode<dh, kv, nhq, false>(p); }                                        \
     extern "C" __global__ __launch_bounds__(256, occ) void g4a_paged_decode_win_d##dh##_##type##_h##nhq(      \
         G4aPagedAttnParams p) { paged_decode<dh, kv, nhq, true>(p); }                                         \
-    extern "C" __global__ __launch_bounds__(256) void g4a_paged_combine16_d##dh##_##type##_h##nhq(            \
-        G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 16>(p); }                                          \
+    extern "C" __global__ __launch_bounds__(1024) void g4a_paged_combine16_d##dh##_##type##_h##nhq(           \
+        G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 16, 16>(p); }                                      \
     extern "C" __global__ __launch_bounds__(256) void g4a_paged_combine64_d##dh##_##type##_h##nhq(            \
-        G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 64>(p); }
+        G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 64, 4>(p); }
 #define G4A_PAGED_DECODE_TYPES(dh, nhq, occ_f32, occ_bf16) \
     G4A_PAGED_DECODE(dh, f32, float, nhq, occ_f32)         \
     G4A_PAGED_DECODE(dh, bf16, __bf16, nhq, occ_bf16)
