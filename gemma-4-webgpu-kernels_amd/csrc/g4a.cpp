@@ -2408,9 +2408,9 @@ int g4a_page_map(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_page_map_
     p.len_out = a->kv_len_out ? a->kv_len_out : cache->kv_len;
     p.state_out = a->free_state_out ? a->free_state_out : a->free_state;
     p.ticket = ctx->ticket;
-    // a workgroup takes 4 rows a thread, and all sequences' scans
+    // a workgroup runs all sequences' scans and takes a row a thread, or more
     const uint32_t threads = cache->n_seqs <= 256 ? 256 : 1024;
-    const uint32_t wgs = std::min<uint32_t>(std::max<uint32_t>(1, (a->rows + 4 * threads - 1) / (4 * threads)),
+    const uint32_t wgs = std::min<uint32_t>(std::max<uint32_t>(1, (a->rows + threads - 1) / threads),
                                             uint32_t(std::max(ctx->cu_count, 1)));
     return launch(ctx, ctx->page_map[threads == 1024], dim3(wgs, 1, 1), dim3(threads, 1, 1), p, "page map", true);
 }
@@ -2487,12 +2487,13 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     // launches of at most PAGED_UNITS units, which bounds the partials' memory, and of as many sequences as
     // the kernel counts
     const uint32_t most = std::min({cache->n_seqs, std::max(1u, PAGED_UNITS / p.units), PAGED_SEQS});
-    // parts: as many as the GPU runs at once, no more of units that leave room for a few parts each, and else
-    // about as many again; none of fewer tiles than there are
+    // Parts: as many as the GPU runs at once, no more of them where that is a few parts a unit, and else
+    // about one a unit more, which leaves as the others end. (One or two workgroups a CU: 96 sequences of
+    // 512 dims 38.8 us, 57.1 beyond what runs at once; four a CU: 512 units of 128 dims 48.6, 42.4.)
     auto shares = [&](uint32_t seqs, uint32_t* spread, uint32_t* fit) {
         const uint64_t units = uint64_t(seqs) * p.units, tiles = uint64_t(p.span / 16 + 2) * units;
         const uint64_t most_parts = std::min<uint64_t>(std::min(resident, PAGED_MAX_PARTS), tiles / PAGED_MIN_PART + units);
-        *fit = 2 * units <= most_parts ? uint32_t(most_parts) : 0;
+        *fit = (PAGED_WGS_PER_CU[d][t][h] >= 3 ? 3 : 2) * units <= most_parts ? uint32_t(most_parts) : 0;
         *spread = uint32_t(std::max<uint64_t>(1, *fit ? most_parts : std::min<uint64_t>(resident, PAGED_MAX_PARTS - 1)));
         return *fit ? *fit : uint32_t(*spread + units);  // the workgroups
     };
@@ -2503,6 +2504,8 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.offs = static_cast<uint32_t*>(ctx->workspace);
     p.part = static_cast<float*>(ctx->workspace) + offs;
     p.part_ml = p.part + size_t(slots) * item;
+    // whether a unit can have more tiles than the smallest part (a window's tokens may start inside a tile)
+    const bool splits = (p.span < p.room ? (p.span + 14) / 16 + 1 : (p.room + 15) / 16) > PAGED_MIN_PART;
     const G4aPagedAttnParams all = p;
     for (uint32_t b0 = 0; b0 < cache->n_seqs; b0 += most) {
         p.c.n_seqs = std::min(most, cache->n_seqs - b0);
@@ -2514,6 +2517,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
         if (int rc = launch(ctx, ctx->paged_decode[a->sliding_window != 0][d][t][h], dim3(wgs, 1, 1), dim3(256, 1, 1), p,
                             "paged decode", true))
             return rc;
+        if (!splits) continue;
         const uint32_t wide = units > PAGED_FEW_UNITS, blocks = uint32_t(item / 4) / (wide ? 64 : 16);
         if (int rc = launch(ctx, ctx->paged_combine[wide][d][t][h], dim3(blocks * units, 1, 1),
                             dim3(wide ? 256 : 1024, 1, 1), p, "paged combine", true))

@@ -103,12 +103,12 @@ __device__ __forceinline__ PagedSpan paged_span(const G4aPagedAttnParams& p, uin
     return s;
 }
 
-// ceil(tiles / quota) parts of a unit, by a reciprocal that is rounded down by 2^-20: exact below
+// ceil(tiles / quota) parts of a unit, one of none (it writes zeros), by a reciprocal that is rounded down by 2^-20: exact below
 // 2^19 tiles, never more. (An integer division each took 2 us of a call of 128 sequences. Every
 // workgroup and the merge compute the same.)
 __device__ __forceinline__ uint32_t paged_parts(uint32_t tiles, uint32_t quota) {
     const float inv = __builtin_amdgcn_rcpf((float)quota) * (1.0f - 0x1p-20f);
-    return tiles ? 1u + (uint32_t)(((float)tiles - 0.5f) * inv) : 0u;
+    return 1u + (uint32_t)fmaxf(((float)tiles - 0.5f) * inv, 0.0f);
 }
 
 // Sums over the lanes up to and with this one: four shifts within the rows of 16 lanes,
@@ -213,10 +213,10 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     uint32_t quota = max((total + p.spread - 1) / p.spread, p.min_part), upto;
     if (quota < 2 * p.min_part) quota = (quota + p.min_part - 1) / p.min_part * p.min_part;  // (whole rounds of the waves)
     // parts of a sequence's units; the first few quotas may give more parts than `fit` holds, the last cannot
-    auto parts_of = [&](uint32_t tiles) { return p.units * paged_parts(tiles, quota); };
+    auto lane_parts = [&](uint32_t b) { return b < n ? p.units * paged_parts(lane_tiles(b), quota) : 0u; };
     for (int tries = 0;; ++tries) {
         mine = 0;
-        for (uint32_t i = 0; i < each; ++i) mine += parts_of(lane_tiles(lane * each + i));
+        for (uint32_t i = 0; i < each; ++i) mine += lane_parts(lane * each + i);
         upto = wave_incl_sum(mine);
         if (p.fit == 0 || (uint32_t)__builtin_amdgcn_readlane(upto, 63) <= p.fit) break;
         const uint32_t sure = (total + p.fit - n * p.units - 1) / (p.fit - n * p.units);
@@ -228,7 +228,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
         for (uint32_t i = 0; i < each; ++i) {
             const uint32_t b = lane * each + i;
             if (b < n) p.offs[1 + b] = before;
-            before += parts_of(lane_tiles(b));
+            before += lane_parts(b);
         }
     }
     const uint32_t at = blockIdx.x;
@@ -240,7 +240,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
         len = __builtin_amdgcn_readlane(my_len, b);
     } else {
         for (const uint32_t last = min(b + each, n);; b += 64) {
-            const uint32_t t = b + lane < last ? parts_of(lane_tiles(b + lane)) : 0u;
+            const uint32_t t = b + lane < last ? lane_parts(b + lane) : 0u;
             const uint32_t u = wave_incl_sum(t);
             const uint64_t hit = __ballot(base + u > at);
             if (hit) {
@@ -255,11 +255,16 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
         barrier_lds();  // every wave has read the lengths: the query rows go there
     }
     const PagedSpan sp = paged_span(p, len);
-    const uint32_t parts = __builtin_amdgcn_readfirstlane(paged_parts(sp.n, quota)), j = (at - base) / parts, part = at - base - j * parts;
+    const uint32_t parts = __builtin_amdgcn_readfirstlane(paged_parts(sp.n, quota));
+    const uint32_t j = (at - base) / parts, part = at - base - j * parts;
     const uint32_t floor = sp.n / parts, more = sp.n % parts;
     const uint32_t s = part * floor + min(part, more), e = s + floor + (part < more ? 1u : 0u);  // its tiles
     const uint32_t kvh = j / p.chunks, h0 = kvh * p.group + (j - kvh * p.chunks) * HR;
     const uint32_t nh = min((uint32_t)HR, p.group - (j - kvh * p.chunks) * HR);
+    if (sp.n == 0) {
+        for (uint32_t i = tid; i < nh * DH; i += 256) p.out[((size_t)b * p.Hq + h0) * DH + i] = 0.0f;
+        return;
+    }
 
     const uint32_t row_bytes = c.Hkv * DH * sizeof(KV);  // (at most 2 MiB)
     // K: lane (g4, key) its key's dims; V: f32 lane LG r + n row KI r, bf16 lane (g4, n) row 4 g4
@@ -591,8 +596,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     }
 }
 
-// Merges the partials of units that more than one workgroup worked on, and writes the
-// zeros of sequences without tokens. A block of W waves takes CI items (4 heads, one
+// Merges the partials of units that more than one workgroup worked on. A block of W waves takes CI items (4 heads, one
 // dim) of a unit, 64 W / CI groups of threads every such part of it: 16 items and 16
 // waves where there are few units of many parts (256 parts of 512 dims: 16 loads a
 // thread on 4 waves took 6.5 us, half of them waiting in turn), 64 items and 4 waves
@@ -619,66 +623,63 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
     static_assert(DH % CI == 0, "a block's items share their heads");
     const uint32_t quota = load_scalar(p.offs, 0), off = load_scalar(p.offs, 1 + b);
     const PagedSpan sp = paged_span(p, load_scalar(p.c.len, b));
-    f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (sp.n) {
-        const uint32_t parts = __builtin_amdgcn_readfirstlane(paged_parts(sp.n, quota)), slot0 = off + j * parts;
-        if (parts == 1) return;
-        const f4v* const part = reinterpret_cast<const f4v*>(p.part) + (size_t)slot0 * C::ITEMS + item;
-        const f4v* const ml = reinterpret_cast<const f4v*>(p.part_ml) + (size_t)slot0 * 2 * NHQ + hq;
-        const f4v none = {G4A_NEG_INF, G4A_NEG_INF, G4A_NEG_INF, G4A_NEG_INF};
-        const bool has = tid < (int)parts;
-        const f4v m0 = has ? ml[(size_t)tid * 2 * NHQ] : none, l0 = has ? ml[(size_t)tid * 2 * NHQ + NHQ] : f4v{};
-        const f4v o0 = gr < (int)parts ? part[(size_t)gr * C::ITEMS] : f4v{};
-        f4v M = m0;
-        for (uint32_t i = tid + NT; i < parts; i += NT)
+    const uint32_t parts = __builtin_amdgcn_readfirstlane(paged_parts(sp.n, quota)), slot0 = off + j * parts;
+    if (parts == 1) return;
+    const f4v* const part = reinterpret_cast<const f4v*>(p.part) + (size_t)slot0 * C::ITEMS + item;
+    const f4v* const ml = reinterpret_cast<const f4v*>(p.part_ml) + (size_t)slot0 * 2 * NHQ + hq;
+    const f4v none = {G4A_NEG_INF, G4A_NEG_INF, G4A_NEG_INF, G4A_NEG_INF};
+    const bool has = tid < (int)parts;
+    const f4v m0 = has ? ml[(size_t)tid * 2 * NHQ] : none, l0 = has ? ml[(size_t)tid * 2 * NHQ + NHQ] : f4v{};
+    const f4v o0 = gr < (int)parts ? part[(size_t)gr * C::ITEMS] : f4v{};
+    f4v M = m0;
+    for (uint32_t i = tid + NT; i < parts; i += NT)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) M[r] = fmaxf(M[r], ml[(size_t)i * 2 * NHQ][r]);
-        // (parts of the first waves only, but for more than NT)
-        const int waves = parts >= NT ? W : (int)(parts + 63) / 64, wave = tid / 64;
-        if (wave < waves) {
+        for (int r = 0; r < 4; ++r) M[r] = fmaxf(M[r], ml[(size_t)i * 2 * NHQ][r]);
+    // (parts of the first waves only, but for more than NT)
+    const int waves = parts >= NT ? W : (int)(parts + 63) / 64, wave = tid / 64;
+    if (wave < waves) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) M[r] = g4a_wave_max(M[r]);
-            if (tid % 64 == 0) r_s[0][wave] = M;
-        }
-        if (waves > 1) {
-            __syncthreads();
-            M = r_s[0][0];
-            for (int i = 1; i < waves; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) M[r] = fmaxf(M[r], r_s[0][i][r]);
-        }
-        f4v L = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (wave < waves) {
-            for (uint32_t i = tid; i < parts; i += NT) {
-                const f4v m = i < NT ? m0 : ml[(size_t)i * 2 * NHQ], l = i < NT ? l0 : ml[(size_t)i * 2 * NHQ + NHQ];
-                f4v f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) f[r] = m[r] == G4A_NEG_INF ? 0.0f : expf(m[r] - M[r]);
-                w_s[i] = f;
-                L += l * f;
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) L[r] = g4a_wave_sum(L[r]);
-            if (tid % 64 == 0) r_s[1][wave] = L;
-        }
-        __syncthreads();
-        if (gr < (int)parts) o = o0 * w_s[gr];
-#pragma unroll 4
-        for (uint32_t i = gr + CG; i < parts; i += CG) o += part[(size_t)i * C::ITEMS] * w_s[i];
-        if constexpr (CI == 16)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = g4a_col_sum4(o[r]);
-        if (tid % 64 < CI) o_s[wave][it] = o;
-        __syncthreads();
-        if (gr) return;
-        L = r_s[1][0];
-        for (int i = 1; i < waves; ++i) L += r_s[1][i];
-#pragma unroll
-        for (int i = 1; i < W; ++i) o += o_s[i][it];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = L[r] != 0.0f ? o[r] / L[r] : 0.0f;
+        for (int r = 0; r < 4; ++r) M[r] = g4a_wave_max(M[r]);
+        if (tid % 64 == 0) r_s[0][wave] = M;
     }
+    if (waves > 1) {
+        __syncthreads();
+        M = r_s[0][0];
+        for (int i = 1; i < waves; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) M[r] = fmaxf(M[r], r_s[0][i][r]);
+    }
+    f4v L = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (wave < waves) {
+        for (uint32_t i = tid; i < parts; i += NT) {
+            const f4v m = i < NT ? m0 : ml[(size_t)i * 2 * NHQ], l = i < NT ? l0 : ml[(size_t)i * 2 * NHQ + NHQ];
+            f4v f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) f[r] = m[r] == G4A_NEG_INF ? 0.0f : expf(m[r] - M[r]);
+            w_s[i] = f;
+            L += l * f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) L[r] = g4a_wave_sum(L[r]);
+        if (tid % 64 == 0) r_s[1][wave] = L;
+    }
+    __syncthreads();
+    f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (gr < (int)parts) o = o0 * w_s[gr];
+#pragma unroll 4
+    for (uint32_t i = gr + CG; i < parts; i += CG) o += part[(size_t)i * C::ITEMS] * w_s[i];
+    if constexpr (CI == 16)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = g4a_col_sum4(o[r]);
+    if (tid % 64 < CI) o_s[wave][it] = o;
+    __syncthreads();
     if (gr) return;
+    L = r_s[1][0];
+    for (int i = 1; i < waves; ++i) L += r_s[1][i];
+#pragma unroll
+    for (int i = 1; i < W; ++i) o += o_s[i][it];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = L[r] != 0.0f ? o[r] / L[r] : 0.0f;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
         if (4 * hq + r < (int)nh) p.out[((size_t)b * p.Hq + h0 + 4 * hq + r) * DH + dim] = o[r];
