@@ -389,6 +389,7 @@ struct G4aPagedProducerParams {
     const uint32_t* slots;      // device [T]; G4A_NO_ROW: no K/V write
     const float* freq;          // [rotary_dim / 2]
     uint32_t T, Hq, heads, rotary_dim;  // heads: rows of a token (Hq, or Hq + 2 Hkv)
+    uint32_t heads_per_wave, groups;    // a token's rows go to `groups` waves
     float eps;
 };
 

@@ -217,10 +217,14 @@ __device__ __forceinline__ void store4(__bf16* p, const f32x4& v) {
 
 // y = rope(x / sqrt(mean(x^2) + eps) * w) for the q, k and v rows of T tokens, in f32: v
 // without w and rotation, q and k unnormalised where w is null. The angle is position *
-// frequency, both f32, as in g4a_norm_rope; its sine and cosine are the device's. The sum
-// of squares is a tree over the row's lanes. K and V rows go to their token's slot.
+// frequency, both f32, as in g4a_norm_rope; its sine and cosine are the device's, once a
+// token and wave. The sum of squares is a tree over the row's lanes. K and V rows go to
+// their token's slot.
 //
-// A row takes DH / 4 lanes (two float4 each at 512), so a wave holds 256 / DH of them.
+// A row takes DH / 4 lanes (two float4 each at 512), so a wave holds 256 / DH of them at a
+// time; it takes heads_per_wave rows of one token, the next rows' loads ahead of the work
+// on these. Bound by HBM in long calls: 16384 tokens of 10 rows of 256 take 67 us (5.0
+// TB/s read and written) with four turns a wave, 89 with one; one token 3.3 us and 5.2.
 constexpr int PP_WAVES = 4;
 
 template <int DH, typename KV>
@@ -228,71 +232,115 @@ __device__ __forceinline__ void paged_producer(const G4aPagedProducerParams& p) 
     constexpr int LPR = DH / 4 < 64 ? DH / 4 : 64;  // lanes of a row
     constexpr int E = DH / (4 * LPR), RPW = 64 / LPR;
     __shared__ __attribute__((aligned(16))) float stage[PP_WAVES][RPW][DH + 4];
-    __shared__ float2 turn[PP_WAVES][RPW][DH / 2];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane / LPR, l = lane % LPR;
+    __shared__ __attribute__((aligned(16))) float2 turn[PP_WAVES][DH / 2];
+    const int lane = threadIdx.x & 63, g = lane / LPR, l = lane % LPR;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const G4aPaged& c = p.c;
-    const uint64_t row = ((uint64_t)blockIdx.x * PP_WAVES + w) * RPW + g;
-    const bool is = row < (uint64_t)p.T * p.heads;
-    const uint32_t t = is ? (uint32_t)(row / p.heads) : 0u, h = is ? (uint32_t)(row - (uint64_t)t * p.heads) : 0u;
-    const uint32_t pos = is ? p.positions[t] : G4A_NO_ROW32;
-    const uint32_t slot = p.heads > p.Hq && is ? p.slots[t] : G4A_NO_ROW32;
-    const bool on_q = h < p.Hq, on_k = !on_q && h < p.Hq + c.Hkv;
-    const uint32_t kvh = on_q ? 0u : (on_k ? h - p.Hq : h - p.Hq - c.Hkv);
-    const bool live = pos != G4A_NO_ROW32 && (on_q || (slot >> c.page_shift) < c.n_pages);
-    const float* const src = on_q   ? p.q + ((size_t)t * p.Hq + h) * DH
-                             : on_k ? p.kx + ((size_t)t * c.Hkv + kvh) * DH
-                                    : p.vx + ((size_t)t * c.Hkv + kvh) * DH;
-    const float* const wt = on_q ? p.q_norm : on_k ? p.k_norm : nullptr;
-    const bool norm = wt || !(on_q || on_k);
-    f32x4 x[E], wv[E];
+    const uint32_t item = blockIdx.x * PP_WAVES + w, t = item / p.groups;
+    if (t >= p.T) return;
+    uint32_t h = (item - t * p.groups) * p.heads_per_wave + g, h_end = min(h - g + p.heads_per_wave, p.heads);
+    // (a branch each: for a choice among pointers the compiler moves the arguments to scratch memory)
+    auto load4 = [&](f32x4 (&x)[E], const float* src) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        x[e] = live ? *reinterpret_cast<const f32x4*>(src + 4 * l + 256 * e) : f32x4{0, 0, 0, 0};
-        wv[e] = live && wt ? *reinterpret_cast<const f32x4*>(wt + 4 * l + 256 * e) : f32x4{1, 1, 1, 1};
-    }
+        for (int e = 0; e < E; ++e) x[e] = *reinterpret_cast<const f32x4*>(src + 4 * l + 256 * e);
+    };
+    auto load = [&](f32x4 (&x)[E], uint32_t h) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = f32x4{0, 0, 0, 0};
+        if (h >= h_end) return;
+        if (h < p.Hq) load4(x, p.q + ((size_t)t * p.Hq + h) * DH);
+        else if (h < p.Hq + c.Hkv) load4(x, p.kx + ((size_t)t * c.Hkv + (h - p.Hq)) * DH);
+        else load4(x, p.vx + ((size_t)t * c.Hkv + (h - p.Hq - c.Hkv)) * DH);
+    };
+    f32x4 x[E], next[E];
+    load(next, h);  // (beside the token's position and slot, not behind them)
+    const uint32_t pos = p.positions[t], slot = p.heads > p.Hq ? p.slots[t] : G4A_NO_ROW32;
+    if (pos == G4A_NO_ROW32) return;
+    if ((slot >> c.page_shift) >= c.n_pages) h_end = min(h_end, p.Hq);
     const uint32_t half = p.rotary_dim / 2;
-    const bool rope = on_q || on_k;
-    if (rope && live)
-        for (uint32_t j = l; j < half; j += LPR) {
-            float sn, cs;
-            sincosf((float)pos * p.freq[j], &sn, &cs);
-            turn[w][g][j] = make_float2(sn, cs);
-        }
-    float ss = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) ss += (x[e].x * x[e].x + x[e].y * x[e].y) + (x[e].z * x[e].z + x[e].w * x[e].w);
-#pragma unroll
-    for (int d = LPR / 2; d > 0; d >>= 1) ss += __shfl_xor(ss, d);
-    const float inv = norm ? 1.0f / sqrtf(ss / (float)DH + p.eps) : 1.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        x[e] = x[e] * inv * wv[e];
-        *reinterpret_cast<f32x4*>(&stage[w][g][4 * l + 256 * e]) = x[e];
+    for (uint32_t j = lane; j < half; j += 64) {
+        float sn, cs;
+        sincosf((float)pos * p.freq[j], &sn, &cs);
+        turn[w][j] = make_float2(sn, cs);
     }
-    __builtin_amdgcn_wave_barrier();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (!live) return;
-    if (rope)
+    for (; h - g < h_end; h += RPW) {  // (lane groups past the last row work on zeros and write nothing)
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = next[e];
+        load(next, h + RPW);
+        const bool on_q = h < p.Hq, on_k = !on_q && h < p.Hq + c.Hkv;
+        const bool norm = on_q ? p.q_norm != nullptr : on_k ? p.k_norm != nullptr : true;
+        f32x4 wv[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) wv[e] = f32x4{1, 1, 1, 1};
+        if (on_q) {
+            if (p.q_norm) load4(wv, p.q_norm);
+        } else if (on_k) {
+            if (p.k_norm) load4(wv, p.k_norm);
+        }
+        float ss = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t d = 4 * l + 256 * e + i;
-                if (d >= p.rotary_dim) continue;
-                const uint32_t j = d < half ? d : d - half;
-                const float a = stage[w][g][j], b = stage[w][g][j + half];
-                const float2 sc = turn[w][g][j];
-                x[e][i] = d < half ? a * sc.y - b * sc.x : b * sc.y + a * sc.x;
+            ss += (x[e].x * x[e].x + x[e].y * x[e].y) + (x[e].z * x[e].z + x[e].w * x[e].w);
+        if constexpr (LPR == 64) {
+            ss = g4a_wave_sum(ss);
+        } else {
+            ss = g4a_row_sum16(ss);
+            if constexpr (LPR == 32) {
+                const float2 y = g4a_pair16(ss);
+                ss = y.x + y.y;
             }
-    if (on_q) {
+        }
+        const float inv = norm ? 1.0f / sqrtf(ss / (float)DH + p.eps) : 1.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) store4(p.q_out + ((size_t)t * p.Hq + h) * DH + 4 * l + 256 * e, x[e]);
-    } else {
-        KV* const pool = reinterpret_cast<KV*>(on_k ? c.k : c.v);
-        const uint32_t page = slot >> c.page_shift, r = slot & ((1u << c.page_shift) - 1);
-        KV* const dst = pool + (size_t)page * c.page_stride + ((size_t)r * c.Hkv + kvh) * DH;
+        for (int e = 0; e < E; ++e) x[e] = x[e] * inv * wv[e];
+        if (half) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) store4(dst + 4 * l + 256 * e, x[e]);
+            for (int e = 0; e < E; ++e) *reinterpret_cast<f32x4*>(&stage[w][g][4 * l + 256 * e]) = x[e];
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (on_q || on_k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const uint32_t d = 4 * l + 256 * e;
+                    if (half % 4 == 0) {  // the lane's four dims are on one side of the pairs
+                        if (d >= p.rotary_dim) continue;
+                        const bool upper = d >= half;
+                        const uint32_t j = upper ? d - half : d;
+                        const f32x4 other = *reinterpret_cast<const f32x4*>(&stage[w][g][upper ? j : j + half]);
+                        const f32x4 sc0 = *reinterpret_cast<const f32x4*>(&turn[w][j]),
+                                    sc1 = *reinterpret_cast<const f32x4*>(&turn[w][j + 2]);
+                        const f32x4 sn = {sc0.x, sc0.z, sc1.x, sc1.z}, cs = {sc0.y, sc0.w, sc1.y, sc1.w};
+                        const f32x4 xc = x[e] * cs, os = other * sn;
+                        x[e] = upper ? xc + os : xc - os;
+                    } else {
+                        auto one = [&](uint32_t d, float y) {
+                            if (d >= p.rotary_dim) return y;
+                            const bool upper = d >= half;
+                            const uint32_t j = upper ? d - half : d;
+                            const float os = stage[w][g][upper ? j : j + half] * turn[w][j].x;
+                            return upper ? y * turn[w][j].y + os : y * turn[w][j].y - os;
+                        };
+                        x[e] = f32x4{one(d, x[e].x), one(d + 1, x[e].y), one(d + 2, x[e].z), one(d + 3, x[e].w)};
+                    }
+                }
+            __builtin_amdgcn_wave_barrier();
+        }
+        if (h >= h_end) continue;
+        if (on_q) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) store4(p.q_out + ((size_t)t * p.Hq + h) * DH + 4 * l + 256 * e, x[e]);
+        } else {
+            const uint32_t kvh = on_k ? h - p.Hq : h - p.Hq - c.Hkv;
+            const uint32_t page = slot >> c.page_shift, r = slot & ((1u << c.page_shift) - 1);
+            const size_t at = (size_t)page * c.page_stride + ((size_t)r * c.Hkv + kvh) * DH + 4 * l;
+            if (on_k) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) store4(reinterpret_cast<KV*>(c.k) + at + 256 * e, x[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) store4(reinterpret_cast<KV*>(c.v) + at + 256 * e, x[e]);
+            }
+        }
     }
 }
 
