@@ -2337,7 +2337,8 @@ constexpr uint32_t PAGED_SEQS = 1024;
 constexpr uint32_t PAGED_FEW_UNITS = 8;
 // Most units of a launch (but for a sequence that has more).
 constexpr uint32_t PAGED_UNITS = 2048;
-// Its workgroups per CU: [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
+// Its workgroups per CU (at 512 dims and up to 8 heads there is room for two, but a call of a few parts a unit is
+// faster with one: 16 ragged sequences of f32 pages 40.9 us, 49.0): [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
 constexpr uint32_t PAGED_WGS_PER_CU[4][2][3] = {
     {{4, 4, 2}, {4, 4, 4}}, {{3, 3, 2}, {4, 4, 3}}, {{2, 2, 1}, {3, 3, 2}}, {{1, 1, 1}, {1, 1, 1}}};
 
@@ -2492,17 +2493,21 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.softcap = a->attn_softcap;
     const int d = paged_dh(cache->Dh), t = int(cache->kv_type);
     const uint32_t resident = uint32_t(std::max(ctx->cu_count, 1)) * PAGED_WGS_PER_CU[d][t][h];
+    // Parts to aim at where there are many units: at 512 dims and up to 8 heads half as many more, which the
+    // second workgroup that a CU has room for takes (256 sequences of up to 1500 tokens, f32: 115 us with them,
+    // 145 without, 129 with as many again; 100 of up to 4000, where there are fewer units, are not concerned).
+    const uint32_t over = d == 3 && h < 2 ? resident + resident / 2 : resident;
     // launches of at most PAGED_UNITS units, which bounds the partials' memory, and of as many sequences as
     // the kernel counts
     const uint32_t most = std::min({cache->n_seqs, std::max(1u, PAGED_UNITS / p.units), PAGED_SEQS});
-    // Parts: as many as the GPU runs at once, no more of them where that is a few parts a unit, and else
-    // about one a unit more, which leaves as the others end. (One or two workgroups a CU: 96 sequences of
+    // Parts: `resident` and no more where that is a few parts a unit, and else about one a unit more, which
+    // leaves as the others end. (One or two workgroups a CU: 96 sequences of
     // 512 dims 38.8 us, 57.1 beyond what runs at once; four a CU: 512 units of 128 dims 48.6, 42.4.)
     auto shares = [&](uint32_t seqs, uint32_t* spread, uint32_t* fit) {
         const uint64_t units = uint64_t(seqs) * p.units, tiles = uint64_t(p.span / 16 + 2) * units;
         const uint64_t most_parts = std::min<uint64_t>(std::min(resident, PAGED_MAX_PARTS), tiles / PAGED_MIN_PART + units);
         *fit = (PAGED_WGS_PER_CU[d][t][h] >= 3 ? 3 : 2) * units <= most_parts ? uint32_t(most_parts) : 0;
-        *spread = uint32_t(std::max<uint64_t>(1, *fit ? most_parts : std::min<uint64_t>(resident, PAGED_MAX_PARTS - 1)));
+        *spread = uint32_t(std::max<uint64_t>(1, *fit ? most_parts : std::min<uint64_t>(over, PAGED_MAX_PARTS - 1)));
         return *fit ? *fit : uint32_t(*spread + units);  // the workgroups
     };
     uint32_t slots = shares(most, &p.spread, &p.fit);

@@ -280,10 +280,12 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
         const uint32_t r = ((sp.first + t) * 16) & ((1u << c.page_shift) - 1);
         return ((size_t)(page < c.n_pages ? page : 0u) * c.page_stride + ((size_t)r * c.Hkv + kvh) * DH) * sizeof(KV);
     };
-    // 16 heads at 512 dims: K and V take turns in one set of registers, V's pieces loaded where K's have
-    // been used and K's next where V's have, as there is no room for both. (With 8 heads, and two workgroups
-    // a CU for it, eight sequences of up to 131072 keys took 146 us, 133 with both in flight.)
-    constexpr bool TURNS = DH == 512 && NHQ == 4;
+    // 512 dims: K and V take turns in one set of registers, V's pieces loaded where K's have been used and
+    // K's next where V's have. With 16 heads there is no room for both; with up to 8 a second workgroup of a
+    // CU starts while the first ends (256 ragged sequences of up to 1500 tokens in bf16 pages: 69.7 us, and
+    // 83.6 with both in flight; one of 32768 in f32 pages 32.6 and 34.5; but eight of up to 131072 in bf16
+    // pages 132.4 and 131.3).
+    constexpr bool TURNS = DH == 512;
     VWord v[C::VL];  // bf16: [row][block of dims]
     u32x4 k_own[TURNS ? 1 : KC];
     u32x4 (&k)[KC] = [&]() -> u32x4 (&)[KC] {
@@ -358,12 +360,20 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
 #pragma unroll
     for (int d = 0; d < NA; ++d) acc[d] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 
+    // The lane, and what follows from it, once more where it is used: kept over the loop those were a few
+    // registers too many, in scratch memory.
+    auto lane_again = [&] {
+        int x = lane;
+        if constexpr (TURNS && NHQ < 4) asm volatile("" : "+v"(x));
+        return x;
+    };
     // One tile; MORE: a piece of the wave's next is loaded where this one's has been used; FIRST: V is
     // loaded between the scores' MFMAs, as ahead of them its loads held up the first of them. (The empty
     // scheduling barriers keep the reads of all query rows, and V's permutes, from being gathered ahead of
     // the first MFMA, in more registers than there are.)
     auto tile = [&](auto first, auto more) {
         constexpr bool FIRST = decltype(first)::value || TURNS, MORE = decltype(more)::value;
+        const int ln = lane_again(), g4 = ln >> 4, key = ln & 15;
         const uint32_t page_after = MORE && t + 8 < e ? page_of(t + 8) : 0u;
         const size_t next = MORE ? tile_at(page_next, t + 4) : 0;
         const PagedTile kt = paged_tile(c.k, next, tile_bytes);
@@ -457,7 +467,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
         if (lo > 0 || hi < 16) {
 #pragma unroll
             for (int i = 0; i < C::VL; ++i) {
-                const uint32_t row = BF ? 4 * g4 + i / C::VB : i / C::LPK + C::KI * (lane / C::LG);
+                const uint32_t row = BF ? 4 * g4 + i / C::VB : i / C::LPK + C::KI * (ln / C::LG);
                 v[i] &= row >= lo && row < hi ? 0xFFFFFFFFu : 0u;
             }
         }
@@ -506,7 +516,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
             __builtin_amdgcn_wave_barrier();
             float pa[NHQ];
 #pragma unroll
-            for (int hq = 0; hq < NHQ; ++hq) pa[hq] = p_s[w][16 * (4 * hq + (lane & 3)) + (lane >> 2)];
+            for (int hq = 0; hq < NHQ; ++hq) pa[hq] = p_s[w][16 * (4 * hq + (ln & 3)) + (ln >> 2)];
             __builtin_amdgcn_wave_barrier();
             auto reload = [&](int ii) {
 #pragma unroll
@@ -531,8 +541,9 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     }
 
     // ---- the waves' partials, through LDS ----
+    const int ln = lane_again(), id = 64 * w + ln;
     l = g4a_col_sum4(l);
-    if (lane < HR) m_s[w][lane] = m, l_s[w][lane] = l;
+    if (ln < HR) m_s[w][ln] = m, l_s[w][ln] = l;
     barrier_lds();  // every wave is done with the query rows, where the accumulators go
 #pragma unroll
     for (int d = 0; d < NA; ++d) {
@@ -547,30 +558,30 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
                 }
             }
         }
-        if (C::ML == 64 || lane < C::ML) mrg[(w * NA + d) * C::ML + lane] = acc[d];
+        if (C::ML == 64 || ln < C::ML) mrg[(w * NA + d) * C::ML + ln] = acc[d];
     }
     const bool whole = parts == 1;
-    if (tid < HR) {
+    if (id < HR) {
         float M = G4A_NEG_INF, L = 0.0f, f[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) M = fmaxf(M, m_s[i][tid]);
+        for (int i = 0; i < 4; ++i) M = fmaxf(M, m_s[i][id]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            f[i] = m_s[i][tid] == G4A_NEG_INF ? 0.0f : expf(m_s[i][tid] - M);
-            L += l_s[i][tid] * f[i];
+            f[i] = m_s[i][id] == G4A_NEG_INF ? 0.0f : expf(m_s[i][id] - M);
+            L += l_s[i][id] * f[i];
         }
         const float inv = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f_s[i][tid] = f[i] * inv;
+        for (int i = 0; i < 4; ++i) f_s[i][id] = f[i] * inv;
         if (!whole) {
-            float* const ml = p.part_ml + (size_t)at * 2 * HR + tid;
+            float* const ml = p.part_ml + (size_t)at * 2 * HR + id;
             ml[0] = M;
             ml[HR] = L;
         }
     }
     barrier_lds();
     f4v* const dst = reinterpret_cast<f4v*>(p.part) + (size_t)at * C::ITEMS;
-    for (int i = tid; i < C::ITEMS; i += 256) {
+    for (int i = id; i < C::ITEMS; i += 256) {
         const int hq = C::hq(i), n = i % C::IL, a = (i / C::IL) % C::IA;
         f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -703,6 +714,6 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
 G4A_PAGED_DECODE_TYPES(64, 1, 4, 4) G4A_PAGED_DECODE_TYPES(64, 2, 4, 4) G4A_PAGED_DECODE_TYPES(64, 4, 2, 4)
 G4A_PAGED_DECODE_TYPES(128, 1, 3, 4) G4A_PAGED_DECODE_TYPES(128, 2, 3, 4) G4A_PAGED_DECODE_TYPES(128, 4, 2, 3)
 G4A_PAGED_DECODE_TYPES(256, 1, 2, 3) G4A_PAGED_DECODE_TYPES(256, 2, 2, 3) G4A_PAGED_DECODE_TYPES(256, 4, 1, 2)
-G4A_PAGED_DECODE_TYPES(512, 1, 1, 1) G4A_PAGED_DECODE_TYPES(512, 2, 1, 1) G4A_PAGED_DECODE_TYPES(512, 4, 1, 1)
+G4A_PAGED_DECODE_TYPES(512, 1, 2, 2) G4A_PAGED_DECODE_TYPES(512, 2, 2, 2) G4A_PAGED_DECODE_TYPES(512, 4, 1, 1)
 #undef G4A_PAGED_DECODE_TYPES
 #undef G4A_PAGED_DECODE
