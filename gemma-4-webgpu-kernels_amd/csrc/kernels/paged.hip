@@ -95,7 +95,7 @@ __device__ __forceinline__ void page_map(const G4aPageMapParams& p) {
     // One pass over all sequences; `rows`: write this workgroup's rows and released
     // pages, `commit`: write the per-sequence outputs and the ring's state.
     auto pass = [&](bool rows, bool commit) {
-        uint32_t row0 = 0;             // rows of the chunks before
+        uint32_t row0 = 0, asked0 = 0;  // rows of the chunks before, and with those refused
         uint32_t need0 = 0, rel0 = 0;  // pages demanded, pages released
         uint32_t taken = 0;            // pages taken
         for (uint32_t b0 = 0; b0 < c.n_seqs; b0 += T) {
@@ -119,9 +119,10 @@ __device__ __forceinline__ void page_map(const G4aPageMapParams& p) {
             uint32_t rn = goes ? want : 0u, gn = goes ? need : 0u, trows, tneed;
             block_scan<T>(rn, gn, trows, tneed, s_sums[1]);
             uint32_t added = goes ? want : 0u, got = goes ? need : 0u;
-            if (p.rows_per_seq == 0 && add_sat(row0, trows) > p.rows) {
+            const uint32_t asked = add_sat(asked0, trows);
+            if (p.rows_per_seq == 0 && asked > p.rows) {
                 // some find no rows: from the first of them on, none that wants any goes
-                if (add_sat(row0, rn) > p.rows) added = got = 0u;
+                if (add_sat(asked0, rn) > p.rows) added = got = 0u;
                 rn = added;
                 gn = got;
                 block_scan<T>(rn, gn, trows, tneed, s_sums[2]);
@@ -178,6 +179,7 @@ __device__ __forceinline__ void page_map(const G4aPageMapParams& p) {
                 }
             }
             row0 += p.rows_per_seq ? 0u : trows;
+            asked0 = asked;
             need0 = add_sat(need0, tn);
             rel0 = add_sat(rel0, tr);
             taken += tneed;

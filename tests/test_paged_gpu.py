@@ -153,6 +153,19 @@ def test_attention_long_and_ragged(ctx, kv_type):
     _check(ctx, [4000] * 9 + [1] * 40 + [900] * 5, 16, "mixed groups", dh=128, hkv=4, kv_type=kv_type, seed=4, cap=20.0)
 
 
+@pytest.mark.parametrize("n,hq,hkv,dh,kv_type,longest", [
+    (2100, 2, 1, 64, "f32", 40), (1025, 8, 1, 64, "bf16", 20), (300, 8, 8, 64, "f32", 70), (150, 40, 5, 128, "bf16", 90),
+    (260, 8, 1, 512, "bf16", 300), (140, 8, 1, 512, "f32", 400), (129, 4, 1, 512, "bf16", 400), (65, 9, 1, 256, "f32", 900)])
+def test_attention_of_many_sequences(ctx, n, hq, hkv, dh, kv_type, longest):
+    """More sequences and head groups than one launch takes, and about as many as run at once; lengths
+    from none to a few parts, one sequence far longer than the others."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, longest + 1, n)
+    lens[[0, n // 2, n - 1]] = [5 * longest, 0, longest]
+    for window in (0, 37):
+        _check(ctx, lens, hq, "many", window=window, hkv=hkv, dh=dh, kv_type=kv_type, seed=n)
+
+
 def test_attention_scale_softcap_and_page_stride(ctx):
     _check(ctx, [100, 513, 31], 8, "scale", dh=256, scale=0.0625, unit=1.0, seed=1)
     _check(ctx, [100, 513, 31], 8, "softcap", dh=512, cap=5.0, unit=1.0, seed=2)
@@ -312,6 +325,18 @@ def test_maps_keep_shared_pages_and_take_single_tokens(ctx):
     _check_map(ctx, "no rows", lens, np.zeros(4, np.uint32), table, free, 0, 3, page=16, ring=False, rows=0)
 
 
+@pytest.mark.parametrize("apart", [False, True])
+def test_maps_refuse_rows_over_thousands_of_sequences(ctx, apart):
+    """Once the rows asked for have passed those there are, no later sequence gets one, however far behind."""
+    n = 2600
+    lens, new = np.zeros(n, np.uint32), np.zeros(n, np.uint32)
+    table = np.full((n, 4), ref.NO_ROW, np.uint32)
+    new[[3, 700, 900, 1030, 1500, 2590]] = [10, 45, 3, 2, 1, 7]
+    free = np.arange(n, dtype=np.uint32)
+    *_, added = _check_map(ctx, "rows", lens, new, table, free, 5, n, page=16, ring=False, rows=50, apart=apart)
+    assert added.sum() == 10
+
+
 def test_maps_of_bad_device_values_stay_inside(ctx):
     """Lengths past the table, a free ring that claims more than it holds, page numbers that do not exist:
     no slot past the pool, nothing written behind the buffers."""
@@ -386,6 +411,13 @@ def test_producer_rows(ctx, dh, rot, theta, kv_type):
     for T, hq, hkv in ((1, 8, 1), (3, 3, 2), (65, 8, 1), (37, 16, 4)):
         say(f"producer T {T} heads {hq}/{hkv} dh {dh} rot {rot} {kv_type}")
         _produce(ctx, T, hq, hkv, dh, kv_type, rot, theta, T + dh)
+
+
+@pytest.mark.parametrize("T,hq,hkv,dh,kv_type", [(1500, 3, 2, 64, "f32"), (1030, 8, 1, 256, "bf16"), (1100, 5, 1, 128, "f32"),
+                                                 (1024, 2, 1, 512, "bf16"), (8200, 4, 1, 64, "bf16"), (8193, 1, 1, 256, "f32")])
+def test_producer_of_long_calls(ctx, T, hq, hkv, dh, kv_type):
+    """Calls whose waves take several rows of a token: numbers of rows that do not divide, tokens without slot or position."""
+    _produce(ctx, T, hq, hkv, dh, kv_type, dh // 2, 1e4, T, skip=[(1, "slot"), (T // 2, "pos"), (T - 2, "past")])
 
 
 def test_producer_variants(ctx):
@@ -545,6 +577,78 @@ def test_a_server_steps_eagerly_and_replayed(ctx, dh, kv_type, window):
         s.step()
         s.check(1)
     graph.free()
+
+
+def test_two_graphs_replay_beside_a_larger_call(ctx):
+    """Two captured calls share the context's workspace, and a later call that needs more of it leaves theirs:
+    replays in any order give what the eager calls gave, as lengths change between them."""
+    c = g4a.Context(0)
+    small, big = (Paged(c, lens, dh=256, kv_type=t, seed=3) for lens, t in (([700, 33, 0], "f32"), ([90, 2000, 17, 5], "bf16")))
+    huge = Paged(c, [3000] * 24, dh=256, hkv=2, seed=4)
+    runs = []
+    for x in (small, big):
+        q = x.queries(8)
+        dq, out = c.upload(q), c.empty((len(q), 8 * 256))
+        runs.append((x, q, dq, out, g4a.PagedAttnArgs(q=dq.ptr, out=out.ptr, Hq=8, scale=1.0)))
+    for x, _, _, _, args in runs:
+        c.attention_paged(x.cache, args)
+    graphs = []
+    for x, _, _, _, args in runs:
+        c.capture_begin()
+        c.attention_paged(x.cache, args)
+        graphs.append(c.capture_end())
+    for turn, (i, cut) in enumerate([(0, 0), (1, 0), (0, 200), (1, 500), (1, 0), (0, 0)]):
+        x, q, _, out, args = runs[i]
+        full = x.lens
+        x.lens = np.maximum(full.astype(np.int64) - cut, 0).astype(np.uint32)
+        c.h2d(x.dlen.ptr, x.lens)
+        if turn == 2:  # a larger workspace, in between
+            hq = huge.queries(16)
+            want, bound = huge.want(hq)
+            _close(huge.attend(hq), want, bound, "the larger call")
+        c.h2d(out.ptr, np.full((len(q), 8 * 256), 7.0, np.float32))
+        graphs[i].launch()
+        want, bound = x.want(q)
+        got = out.to_host()
+        _close(got, want, bound, f"replay {turn}")
+        c.attention_paged(x.cache, args)
+        assert np.array_equal(out.to_host(), got), "the eager call's bits"
+        x.lens = full
+    for g in graphs:
+        g.free()
+    c.close()
+
+
+@pytest.mark.parametrize("kv_type", ["f32", "bf16"])
+def test_pages_past_four_gib(ctx, kv_type):
+    """The same tokens in pages side by side and more than 2^32 bytes apart: produced, gathered and attended alike, bit for bit."""
+    size = 4 if kv_type == "f32" else 2
+    T, page, dh, far = 90, 32, 256, (1 << 32) // size + 64
+    rng = np.random.default_rng(8)
+    x = {m: ctx.upload(rng.standard_normal((T, h, dh)).astype(np.float32)) for m, h in (("q", 8), ("k", 1), ("v", 1))}
+    table, slots = np.array([[2, 0, 1]], np.uint32), np.zeros(T, np.uint32)
+    t = np.arange(T)
+    slots[:] = table[0, t // page] * page + t % page
+    d = dict(table=ctx.upload(table), len=ctx.upload(np.array([T], np.uint32)), slots=ctx.upload(slots),
+             pos=ctx.upload(t.astype(np.uint32)))
+    got = []
+    for stride in (page * dh, far):
+        pools = [ctx.empty(((2 * stride + page * dh) * size // 4,)) for _ in range(2)]
+        q, out, k, v = (ctx.empty(s) for s in ((T, 8, dh), (1, 8 * dh), (T, 1, dh), (T, 1, dh)))
+        cache = g4a.PagedCache(k_pages=pools[0].ptr, v_pages=pools[1].ptr, block_table=d["table"].ptr, kv_len=d["len"].ptr,
+                               page_stride=stride, n_seqs=1, pages_per_seq=3, n_pages=3, page_size=page, Hkv=1, Dh=dh,
+                               kv_type=g4a.KV_TYPES[kv_type])
+        say(f"stride {stride} {kv_type}")
+        ctx.attn_producer_paged(cache, g4a.PagedProducerArgs(q=x["q"].ptr, k=x["k"].ptr, v=x["v"].ptr, q_out=q.ptr,
+                                                             positions=d["pos"].ptr, slots=d["slots"].ptr, T=T, Hq=8,
+                                                             rotary_dim=dh, theta=1e4, eps=1e-6))
+        ctx.kv_gather_paged(cache, 0, 0, T, k.ptr, v.ptr)
+        ctx.attention_paged(cache, g4a.PagedAttnArgs(q=q.ptr, out=out.ptr, Hq=8, scale=0.1))
+        got.append([y.to_host() for y in (k, v, out)])
+        for y in (*pools, q, out, k, v):
+            y.free()
+    assert all(np.isfinite(y).all() and y.any() for y in got[0])
+    assert all(np.array_equal(a, b) for a, b in zip(*got))
 
 
 def test_a_prompt_continues_a_cached_prefix(ctx):

@@ -142,6 +142,35 @@ def test_a_rotation_is_first_used_outside_a_capture(ctx):
     ctx.capture_end().free()
 
 
+def test_attention_launches(ctx):
+    """What a call launches follows from its arguments: one decode and one merge kernel a launch of up to 1024
+    sequences and 2048 head groups, no merge where no sequence can have more than the smallest part."""
+    def names(**kw):
+        attn = {k: kw.pop(k) for k in ("Hq", "sliding_window") if k in kw}
+        ctx.attention_paged(_cache(**kw), _attn(**attn))
+        return [x.name for x in hip.launches()]
+
+    assert names(Dh=512) == ["g4a_paged_decode_d512_f32_h2", "g4a_paged_combine16_d512_f32_h2"]
+    assert names(n_seqs=9, kv_type=1, Hq=4) == ["g4a_paged_decode_d256_bf16_h1", "g4a_paged_combine64_d256_bf16_h1"]
+    assert names(sliding_window=100, Hq=9) == ["g4a_paged_decode_win_d256_f32_h4", "g4a_paged_combine16_d256_f32_h4"]
+    # 50 tokens from the last row of a tile of 16 on touch five tiles (1 + 16 + 16 + 16 + 1), 49 at most four
+    assert names(sliding_window=50) == ["g4a_paged_decode_win_d256_f32_h2", "g4a_paged_combine16_d256_f32_h2"]
+    assert names(sliding_window=49) == ["g4a_paged_decode_win_d256_f32_h2"]
+    assert names(pages_per_seq=4) == ["g4a_paged_decode_d256_f32_h2"]
+    assert len(names(n_seqs=2100)) == 6 and len(names(n_seqs=1024)) == 2
+    assert len(names(n_seqs=600, Hkv=4, Hq=32)) == 4
+
+
+def test_attention_grows_its_workspace_outside_a_capture(ctx):
+    ctx.attention_paged(_cache(), _attn())
+    ctx.capture_begin()
+    ctx.attention_paged(_cache(), _attn())
+    with pytest.raises(hip.binding().G4aError, match="capture"):
+        ctx.attention_paged(_cache(n_seqs=600, Dh=512, pages_per_seq=64), _attn())
+    with pytest.raises(hip.binding().G4aError):
+        ctx.capture_end()
+
+
 def test_the_reference_map_keeps_every_page_once():
     """Steps of random demands: pages are owned by one sequence or free, never both, and
     slots of live tokens differ."""
