@@ -2533,7 +2533,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
         if (!splits) continue;
         const uint32_t wide = units > PAGED_FEW_UNITS, blocks = uint32_t(item / 4) / (wide ? 64 : 16);
         if (int rc = launch(ctx, ctx->paged_combine[wide][d][t][h], dim3(blocks * units, 1, 1),
-                            dim3(wide ? 256 : 1024, 1, 1), p, "paged combine", true))
+                            dim3(wide ? 256 : 512, 1, 1), p, "paged combine", true))
             return rc;
     }
     return G4A_OK;

@@ -210,8 +210,8 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     uint32_t mine = 0;
     for (uint32_t i = 0; i < each; ++i) mine += lane_tiles(lane * each + i);
     const uint32_t total = (uint32_t)__builtin_amdgcn_readlane(wave_incl_sum(mine), 63) * p.units;
+    // (not in whole rounds of the waves: 64 windows of 512, hd 256 f32, took 23.4 us so, 21.1 with parts of five tiles)
     uint32_t quota = max((total + p.spread - 1) / p.spread, p.min_part), upto;
-    if (quota < 2 * p.min_part) quota = (quota + p.min_part - 1) / p.min_part * p.min_part;  // (whole rounds of the waves)
     // parts of a sequence's units; the first few quotas may give more parts than `fit` holds, the last cannot
     auto lane_parts = [&](uint32_t b) { return b < n ? p.units * paged_parts(lane_tiles(b), quota) : 0u; };
     for (int tries = 0;; ++tries) {
@@ -608,10 +608,10 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
 }
 
 // Merges the partials of units that more than one workgroup worked on. A block of W waves takes CI items (4 heads, one
-// dim) of a unit, 64 W / CI groups of threads every such part of it: 16 items and 16
-// waves where there are few units of many parts (256 parts of 512 dims: 16 loads a
-// thread on 4 waves took 6.5 us, half of them waiting in turn), 64 items and 4 waves
-// where there are many units. A thread's first partial is loaded with the parts' maxima
+// dim) of a unit, 64 W / CI groups of threads every such part of it: 16 items and 8
+// waves where there are few units of many parts (256 parts of 512 dims: with 64 items
+// and 4 waves a call took 36.9 us, 32.5 so; a window of 512 on 4, 8, 16 waves 11.1, 11.2,
+// 11.6), 64 items and 4 waves where there are many units. A thread's first partial is loaded with the parts' maxima
 // and sums, ahead of the weights e^(m - M), which are computed a part a thread and meet
 // in LDS.
 constexpr int PAGED_PARTS = 1024;  // of a unit, at most
@@ -703,8 +703,8 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
         G4aPagedAttnParams p) { paged_decode<dh, kv, nhq, false>(p); }                                        \
     extern "C" __global__ __launch_bounds__(256, occ) void g4a_paged_decode_win_d##dh##_##type##_h##nhq(      \
         G4aPagedAttnParams p) { paged_decode<dh, kv, nhq, true>(p); }                                         \
-    extern "C" __global__ __launch_bounds__(1024) void g4a_paged_combine16_d##dh##_##type##_h##nhq(           \
-        G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 16, 16>(p); }                                      \
+    extern "C" __global__ __launch_bounds__(512) void g4a_paged_combine16_d##dh##_##type##_h##nhq(            \
+        G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 16, 8>(p); }                                      \
     extern "C" __global__ __launch_bounds__(256) void g4a_paged_combine64_d##dh##_##type##_h##nhq(            \
         G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 64, 4>(p); }
 #define G4A_PAGED_DECODE_TYPES(dh, nhq, occ_f32, occ_bf16) \
