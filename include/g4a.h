@@ -407,7 +407,8 @@ int g4a_embed_rows_q(g4a_ctx *ctx, const g4a_qweight *table, const uint32_t *ids
  * it on the context's stream with the same pointers and arguments.
  * Capturable: attention with contiguous positions (q_pos0 / k_pos0), the
  * producer and norm/RoPE calls with contiguous positions, kv_write, every
- * projection, elementwise and norm op. A call that needs host staging
+ * projection, elementwise and norm op, and the paged cache's four calls. A call
+ * that needs host staging
  * (explicit position arrays, embedding ids), a larger workspace or a new RoPE
  * table, and g4a_h2d / g4a_d2h / g4a_zero / g4a_sync / the timers, fail with
  * G4A_E_ARG while a capture is open: run such calls once before capturing.
@@ -537,6 +538,7 @@ typedef struct g4a_paged_cache {
  * free_cap must hold all pages that can be free at once. kv_len_out and
  * free_state_out receive the lengths and the state after the step, NULL:
  * cache->kv_len and free_state themselves; table and ring are written in place.
+ * No two buffers of a call overlap otherwise.
  * The cache's pools and widths are not looked at. */
 typedef struct g4a_page_map_args {
     const uint32_t *new_len;      /* device [n_seqs], or NULL: one token each */
@@ -585,7 +587,9 @@ int g4a_attn_producer_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4
  * sliding_window tokens (0: all; a ring: at most those it holds), with scale and
  * soft-cap as in g4a_attention; zeros where kv_len[b] is 0. Query head h reads kv
  * head h / (Hq / Hkv). Every kernel and grid depends on the arguments alone, so a
- * captured call follows lengths and tables. */
+ * captured call follows lengths and tables. The partial results of sequences that
+ * several workgroups share stand in the context's workspace: run the call once, at
+ * its sizes, before capturing it. Results are the same bits from call to call. */
 typedef struct g4a_paged_attn_args {
     const float *q; /* [n_seqs, Hq, Dh], 16-byte aligned */
     float *out;     /* [n_seqs, Hq * Dh], 16-byte aligned */
@@ -610,8 +614,9 @@ int g4a_timer_stop(g4a_ctx *ctx, float *ms);
 /* Per-kernel timing: while enabled, every g4a_attention call records a HIP
  * event pair on the context's stream around its main kernel (decode, prefill
  * or generic; not the LSE combine), and so does every norm/RoPE/producer
- * launch, every decode and combine launch of g4a_attention_decode_batch and
- * every quantised projection / embedding launch.
+ * launch, every decode and combine launch of g4a_attention_decode_batch, every
+ * launch of the paged cache's calls and every quantised projection / embedding
+ * launch.
  * g4a_kernel_timing_read waits for the
  * recorded pairs and returns their summed milliseconds and count, then clears
  * them. At most 4096 pairs are kept per read. Enabling clears old pairs. */
