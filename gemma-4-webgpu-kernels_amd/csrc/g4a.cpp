@@ -928,11 +928,6 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
         snprintf(name, sizeof name, "g4a_paged_gather_%s", type);
         if (int rc = get_fn(ctx, &ctx->paged_gather[t], name)) return bail(rc);
     }
-    if (hipMalloc(reinterpret_cast<void**>(&ctx->ticket), 256) != hipSuccess ||
-        hipMemset(ctx->ticket, 0, 256) != hipSuccess) {
-        fail(ctx, G4A_E_NOMEM, "ticket allocation failed");
-        return bail(G4A_E_NOMEM);
-    }
     if (hipMalloc(reinterpret_cast<void**>(&ctx->dummy), 4096) != hipSuccess ||
         hipMemset(ctx->dummy, 0, 4096) != hipSuccess) {
         fail(ctx, G4A_E_NOMEM, "dummy buffer allocation failed");
@@ -944,6 +939,12 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
         hipEventCreateWithFlags(&ctx->ev_staging, hipEventDisableTiming) != hipSuccess) {
         fail(ctx, G4A_E_HIP, "stream/event creation failed");
         return bail(G4A_E_HIP);
+    }
+    // on the context's own stream, ahead of its launches
+    if (hipMalloc(reinterpret_cast<void**>(&ctx->ticket), 256) != hipSuccess ||
+        hipMemsetAsync(ctx->ticket, 0, 256, ctx->stream) != hipSuccess) {
+        fail(ctx, G4A_E_NOMEM, "ticket allocation failed");
+        return bail(G4A_E_NOMEM);
     }
     *out = ctx;
     return G4A_OK;
@@ -2335,10 +2336,13 @@ constexpr uint32_t PAGED_MAX_PARTS = 1024;
 constexpr uint32_t PAGED_SEQS = 1024;
 // Units up to which a merge block takes 16 items of one, not 64.
 constexpr uint32_t PAGED_FEW_UNITS = 8;
+// Most workgroups of 256 threads of a launch: their threads along x are counted in 32 bits.
+constexpr uint32_t PAGED_GRID = 0xFFFFFF;
 // Most units of a launch (but for a sequence that has more).
 constexpr uint32_t PAGED_UNITS = 2048;
-// Its workgroups per CU (at 512 dims and up to 8 heads there is room for two, but a call of a few parts a unit is
-// faster with one: 16 ragged sequences of f32 pages 40.9 us, 49.0): [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
+// Its workgroups per CU (at 512 dims and up to 8 heads there is room for two, but a call of a few parts a
+// unit is faster with one: 16 ragged sequences of f32 pages 40.9 us, 49.0):
+// [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
 constexpr uint32_t PAGED_WGS_PER_CU[4][2][3] = {
     {{4, 4, 2}, {4, 4, 4}}, {{3, 3, 2}, {4, 4, 3}}, {{2, 2, 1}, {3, 3, 2}}, {{1, 1, 1}, {1, 1, 1}}};
 
@@ -2428,13 +2432,22 @@ int g4a_attn_producer_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4
     if (a->Hq == 0 || a->Hq > 65536) return fail(ctx, G4A_E_UNSUPPORTED, "Hq %u is not 1 .. 65536", a->Hq);
     p.heads = a->Hq + (a->k ? 2 * cache->Hkv : 0);
     const uint64_t rows = uint64_t(a->T) * p.heads;
-    if (rows >> 32) return fail(ctx, G4A_E_SHAPE, "too many rows (%llu)", (unsigned long long)rows);
     if (a->T == 0) return G4A_OK;
     if (!a->q || !a->q_out || !a->positions || (a->k && !a->slots))
         return fail(ctx, G4A_E_ARG, "null q / q_out / positions / slots");
     for (const void* x : {(const void*)a->q, (const void*)a->k, (const void*)a->v, (const void*)a->q_norm,
                           (const void*)a->k_norm, (const void*)a->q_out})
         if (!aligned16(x)) return fail(ctx, G4A_E_ARG, "rows and norm weights must be 16-byte aligned");
+    // More rows of a token to a wave share its sines and their loads overlap, but fewer waves run
+    // at once (4099 tokens of 10 rows of 256: 21.8, 18.3, 18.2 us with 1, 2, 5 turns a wave; 16384:
+    // 88.8, 73.0, 64.6, and 67.2 with 4; 512: 4.9, 5.2, 6.6). A row of 512 is two loads a lane already.
+    const uint32_t at_once = std::max<uint32_t>(1, 256 / cache->Dh);  // rows a wave holds
+    const uint32_t cus = uint32_t(std::max(ctx->cu_count, 1));
+    const uint32_t turns = a->T < 4 * cus ? 1 : a->T < 32 * cus || cache->Dh > 256 ? 2 : 4;
+    p.heads_per_wave = turns * at_once;
+    p.groups = (p.heads + p.heads_per_wave - 1) / p.heads_per_wave;
+    const uint64_t wgs = (uint64_t(a->T) * p.groups + 3) / 4;
+    if (wgs > PAGED_GRID) return fail(ctx, G4A_E_SHAPE, "too many rows (%llu)", (unsigned long long)rows);
     if (rot)
         if (int rc = freq_table(ctx, a->theta, rot, &p.freq)) return rc;
     p.q = a->q;
@@ -2449,16 +2462,7 @@ int g4a_attn_producer_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4
     p.Hq = a->Hq;
     p.rotary_dim = rot;
     p.eps = a->eps;
-    // More rows of a token to a wave share its sines and their loads overlap, but fewer waves run
-    // at once (4099 tokens of 10 rows of 256: 21.8, 18.3, 18.2 us with 1, 2, 5 turns a wave; 16384:
-    // 88.8, 73.0, 64.6, and 67.2 with 4; 512: 4.9, 5.2, 6.6). A row of 512 is two loads a lane already.
-    const uint32_t at_once = std::max<uint32_t>(1, 256 / cache->Dh);  // rows a wave holds
-    const uint32_t cus = uint32_t(std::max(ctx->cu_count, 1));
-    const uint32_t turns = a->T < 4 * cus ? 1 : a->T < 32 * cus || cache->Dh > 256 ? 2 : 4;
-    p.heads_per_wave = turns * at_once;
-    p.groups = (p.heads + p.heads_per_wave - 1) / p.heads_per_wave;
-    const uint64_t waves = uint64_t(a->T) * p.groups;
-    return launch(ctx, ctx->paged_producer[paged_dh(cache->Dh)][cache->kv_type], dim3(uint32_t((waves + 3) / 4), 1, 1),
+    return launch(ctx, ctx->paged_producer[paged_dh(cache->Dh)][cache->kv_type], dim3(uint32_t(wgs), 1, 1),
                   dim3(256, 1, 1), p, "paged producer", true);
 }
 
@@ -2501,8 +2505,8 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     // the kernel counts
     const uint32_t most = std::min({cache->n_seqs, std::max(1u, PAGED_UNITS / p.units), PAGED_SEQS});
     // Parts: `resident` and no more where that is a few parts a unit, and else about one a unit more, which
-    // leaves as the others end. (One or two workgroups a CU: 96 sequences of
-    // 512 dims 38.8 us, 57.1 beyond what runs at once; four a CU: 512 units of 128 dims 48.6, 42.4.)
+    // leaves as the others end. (One or two workgroups a CU: 96 sequences of 512 dims 38.8 us, 57.1 beyond
+    // what runs at once; four a CU: 512 units of 128 dims 48.6, 42.4.)
     auto shares = [&](uint32_t seqs, uint32_t* spread, uint32_t* fit) {
         const uint64_t units = uint64_t(seqs) * p.units, tiles = uint64_t(p.span / 16 + 2) * units;
         const uint64_t most_parts = std::min<uint64_t>(std::min(resident, PAGED_MAX_PARTS), tiles / PAGED_MIN_PART + units);
@@ -2557,6 +2561,8 @@ int g4a_kv_gather_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, uint32_t seq
     // about 16 KiB of rows a workgroup
     while (p.rows_shift < p.c.page_shift && (uint64_t(cache->Hkv) * cache->Dh * 4 << p.rows_shift) < 16384) ++p.rows_shift;
     const uint32_t groups = ((pos0 + n - 1) >> p.rows_shift) - (pos0 >> p.rows_shift) + 1;
+    if (groups > PAGED_GRID)
+        return fail(ctx, G4A_E_SHAPE, "%u tokens: a gather takes %u groups of %u", n, PAGED_GRID, 1u << p.rows_shift);
     return launch(ctx, ctx->paged_gather[cache->kv_type], dim3(groups, 2, 1), dim3(256, 1, 1), p, "paged gather", true);
 }
 

@@ -118,6 +118,18 @@ def test_bad_gathers_are_refused(ctx, code, text, args):
     _refused(ctx, code, text, ctx.kv_gather_paged, _cache(), *args)
 
 
+def test_calls_past_a_launch_are_refused(ctx):
+    """A launch counts its threads in 32 bits: 2^24 - 1 workgroups of 256. At 512 dims a wave takes two rows of a
+    token, four waves a workgroup; a gather of 64-dim rows takes a page of 16 a workgroup."""
+    most = (1 << 24) - 1
+    ctx.attn_producer_paged(_cache(Dh=512), _producer(T=4 * most // 5))
+    assert [x.gx for x in hip.launches()] == [(4 * most // 5 * 5 + 3) // 4]
+    _refused(ctx, SHAPE, "rows", ctx.attn_producer_paged, _cache(Dh=512), _producer(T=4 * most // 5 + 1))
+    ctx.kv_gather_paged(_cache(Dh=64), 0, 0, 16 * most, PTR, PTR)
+    assert [x.gx for x in hip.launches()] == [most]
+    _refused(ctx, SHAPE, "groups", ctx.kv_gather_paged, _cache(Dh=64), 0, 0, 16 * most + 1, PTR, PTR)
+
+
 def test_calls_without_work_launch_nothing(ctx):
     ctx.page_map(_cache(n_seqs=0), _map(rows=0))
     ctx.attn_producer_paged(_cache(), _producer(T=0))
