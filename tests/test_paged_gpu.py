@@ -337,6 +337,43 @@ def test_maps_refuse_rows_over_thousands_of_sequences(ctx, apart):
     assert added.sum() == 10
 
 
+def test_maps_in_place_replay_over_many_workgroups(ctx):
+    """One captured step of thousands of rows, lengths and free ring in place, replayed with other demands, an
+    eager step between the replays: each leaves what a walk over the sequences leaves."""
+    rng = np.random.default_rng(12)
+    n, per_seq, page, rows, cap = 300, 12, 16, 6000, 2500
+    lens, table = np.zeros(n, np.uint32), np.full((n, per_seq), ref.NO_ROW, np.uint32)
+    free, first, count = rng.permutation(cap).astype(np.uint32), 7, cap
+    d = {k: ctx.upload(np.ascontiguousarray(v, np.uint32)) for k, v in dict(
+        lens=lens, new=np.zeros(n), table=table, free=free, state=[first, count], slots=np.zeros(rows),
+        pos=np.zeros(rows), start=np.zeros(n + 1), added=np.zeros(n)).items()}
+    cache = g4a.PagedCache(block_table=d["table"].ptr, kv_len=d["lens"].ptr, n_seqs=n, pages_per_seq=per_seq, n_pages=cap,
+                           page_size=page)
+    args = g4a.PageMapArgs(new_len=d["new"].ptr, free_pages=d["free"].ptr, free_state=d["state"].ptr, slots=d["slots"].ptr,
+                           positions=d["pos"].ptr, row_start=d["start"].ptr, added=d["added"].ptr, free_cap=cap, rows=rows)
+    ctx.capture_begin()
+    ctx.page_map(cache, args)
+    graph = ctx.capture_end()
+    for step in range(8):
+        new = rng.integers(0, 40, n).astype(np.uint32)
+        new[rng.random(n) < 0.2] = ref.NO_ROW if step % 3 else 1
+        ctx.h2d(d["new"].ptr, new)
+        if step % 4 == 2:
+            ctx.page_map(cache, args)
+        else:
+            graph.launch()
+        say(f"step {step}")
+        slots, pos, start, added, lens, table, free, first, count = ref.page_map(
+            lens, new, table, free, first, count, page=page, ring=False, rows=rows)
+        want = dict(slots=slots, pos=pos, start=start, added=added, lens=lens, table=table, free=free,
+                    state=np.array([first, count]))
+        for k, v in want.items():
+            assert np.array_equal(d[k].to_host(), v), (step, k)
+    graph.free()
+    for v in d.values():
+        v.free()
+
+
 def test_maps_of_bad_device_values_stay_inside(ctx):
     """Lengths past the table, a free ring that claims more than it holds, page numbers that do not exist:
     no slot past the pool, nothing written behind the buffers."""
