@@ -2521,8 +2521,9 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.offs = static_cast<uint32_t*>(ctx->workspace);
     p.part = static_cast<float*>(ctx->workspace) + offs;
     p.part_ml = p.part + size_t(slots) * item;
-    // whether a unit can have more tiles than the smallest part (a window's tokens may start inside a tile)
-    const bool splits = (p.span < p.room ? (p.span + 14) / 16 + 1 : (p.room + 15) / 16) > PAGED_MIN_PART;
+    // whether a unit can have more tiles than the smallest part (a window's tokens may start inside a tile, and so
+    // may a ring's)
+    const bool splits = (p.span < p.room || cache->ring ? (p.span + 14) / 16 + 1 : (p.room + 15) / 16) > PAGED_MIN_PART;
     const G4aPagedAttnParams all = p;
     for (uint32_t b0 = 0; b0 < cache->n_seqs; b0 += most) {
         p.c.n_seqs = std::min(most, cache->n_seqs - b0);

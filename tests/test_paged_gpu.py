@@ -146,6 +146,16 @@ def test_attention_windows_and_rings(ctx, window, kv_type):
 
 
 @pytest.mark.parametrize("kv_type", ["f32", "bf16"])
+@pytest.mark.parametrize("page,per_seq", [(16, 4), (32, 2), (64, 1), (16, 3), (16, 5)])
+def test_attention_over_rings_of_about_a_part(ctx, page, per_seq, kv_type):
+    """A ring of four tiles, the smallest part, shows 64 tokens that touch five where they start inside one."""
+    for lens in ([65], [0, 1, 48, 49, 63, 64, 65, 70, 79, 80, 100, 1000]):
+        for window in (0, 63, 64, 100):
+            _check(ctx, lens, 8, f"ring {page} x {per_seq}", window=window, dh=256, kv_type=kv_type, page=page, ring=True,
+                   per_seq=per_seq, seed=per_seq + window)
+
+
+@pytest.mark.parametrize("kv_type", ["f32", "bf16"])
 def test_attention_long_and_ragged(ctx, kv_type):
     _check(ctx, [20011], 8, "one long", dh=512, kv_type=kv_type, page=64, seed=1)
     _check(ctx, [9001, 3, 0, 4097, 1, 700, 12000], 8, "ragged", dh=256, kv_type=kv_type, seed=2)

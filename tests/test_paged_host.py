@@ -173,6 +173,22 @@ def test_attention_launches(ctx):
     assert len(names(n_seqs=600, Hkv=4, Hq=32)) == 4
 
 
+@pytest.mark.parametrize("window", [0, 64, 100])
+@pytest.mark.parametrize("page,per_seq", [(16, 4), (32, 2), (64, 1)])
+def test_a_ring_of_four_tiles_is_merged(ctx, page, per_seq, window):
+    """64 tokens of a ring touch five tiles where the first of them is inside one; a table that is no ring starts
+    with its first tile, and a ring of 48 touches four at most."""
+    def names(ring, per_seq):
+        ctx.attention_paged(_cache(page_size=page, pages_per_seq=per_seq, ring=ring), _attn(sliding_window=window))
+        return [x.name for x in hip.launches()]
+
+    decode = "g4a_paged_decode_win_d256_f32_h2" if window else "g4a_paged_decode_d256_f32_h2"
+    assert names(1, per_seq) == [decode, "g4a_paged_combine16_d256_f32_h2"]
+    assert names(0, per_seq) == [decode]
+    if page == 16:
+        assert names(1, 3) == [decode]
+
+
 def test_attention_grows_its_workspace_outside_a_capture(ctx):
     ctx.attention_paged(_cache(), _attn())
     ctx.capture_begin()
