@@ -2395,7 +2395,7 @@ int g4a_page_map(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_page_map_
     if (a->rows_per_seq && uint64_t(a->rows_per_seq) * cache->n_seqs != a->rows)
         return fail(ctx, G4A_E_SHAPE, "%u rows are not %u for each of %u sequences", a->rows, a->rows_per_seq,
                     cache->n_seqs);
-    if (cache->n_seqs == 0 && a->rows == 0) return G4A_OK;
+    if (cache->n_seqs == 0 && a->rows == 0 && !a->row_start && !a->free_state_out) return G4A_OK;
     if (a->rows && (!a->slots || !a->positions)) return fail(ctx, G4A_E_ARG, "null slots / positions");
     if (!a->free_pages || !a->free_state || a->free_cap == 0)
         return fail(ctx, G4A_E_ARG, "null free_pages / free_state or an empty free ring");

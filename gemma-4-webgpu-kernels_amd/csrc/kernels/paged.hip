@@ -140,8 +140,6 @@ __device__ __forceinline__ void page_map(const G4aPageMapParams& p) {
             if (commit && is) {
                 if (p.added) p.added[b] = added;
                 if (p.row_start) p.row_start[b] = p.rows_per_seq ? b * p.rows_per_seq : row_end - added;
-                if (p.row_start && b + 1 == c.n_seqs)
-                    p.row_start[c.n_seqs] = p.rows_per_seq ? c.n_seqs * p.rows_per_seq : row_end;
                 p.len_out[b] = ends ? 0u : len + added;
             }
             if (rows) {
@@ -190,6 +188,7 @@ __device__ __forceinline__ void page_map(const G4aPageMapParams& p) {
                 p.positions[r] = G4A_NO_ROW32;
             }
         if (commit && tid == 0) {
+            if (p.row_start) p.row_start[c.n_seqs] = p.rows_per_seq ? c.n_seqs * p.rows_per_seq : row0;
             p.state_out[0] = place(taken);
             p.state_out[1] = min(add_sat(count - taken, rel0), cap);
         }

@@ -396,6 +396,28 @@ def test_maps_of_bad_device_values_stay_inside(ctx):
     assert (live < 8 * 16).all() and (got["slots"][40:] == 9).all()
 
 
+@pytest.mark.parametrize("apart", [False, True])
+def test_a_map_of_no_sequence(ctx, apart):
+    """Without a sequence no row has a token: row_start is its end alone, 0, and the ring's state goes on."""
+    for rows in (0, 5, 70000):
+        say(f"no sequence, {rows} rows, apart {apart}")
+        d = {k: ctx.upload(np.asarray(v, np.uint32)) for k, v in dict(
+            free=[4, 2, 7], state=[5, 2], slots=np.full(rows + 5, 9), pos=np.full(rows + 5, 9), start=[9, 9],
+            state2=[9, 9, 9]).items()}
+        args = g4a.PageMapArgs(free_pages=d["free"].ptr, free_state=d["state"].ptr, slots=d["slots"].ptr,
+                               positions=d["pos"].ptr, row_start=d["start"].ptr,
+                               free_state_out=d["state2"].ptr if apart else None, free_cap=3, rows=rows)
+        ctx.page_map(g4a.PagedCache(n_pages=8, page_size=16), args)
+        got = {k: list(v.to_host()) for k, v in d.items()}
+        assert got["start"] == [0, 9] and got["free"] == [4, 2, 7]
+        assert got["state2" if apart else "state"][:2] == [2, 2]  # (place 5 of a ring of 3 is place 2)
+        assert got["state2"][2] == 9 and (not apart or got["state"] == [5, 2])
+        for k in ("slots", "pos"):
+            assert got[k] == [ref.NO_ROW] * rows + [9] * 5
+        for v in d.values():
+            v.free()
+
+
 # ---- the producer ------------------------------------------------------------------
 
 def _produce(ctx, T, hq, hkv, dh, kv_type, rot, theta, seed, *, norms=True, kv=True, page=16, stride=0, pos=None,

@@ -138,6 +138,13 @@ def test_calls_without_work_launch_nothing(ctx):
     assert hip.launches() == []
 
 
+def test_a_map_of_no_sequence_still_gives_its_end_and_the_ring_state(ctx):
+    for kw in (dict(row_start=PTR), dict(free_state_out=PTR + 256)):
+        ctx.page_map(_cache(n_seqs=0, block_table=None, kv_len=None), _map(rows=0, **kw))
+        assert [x.name for x in hip.launches()] == ["g4a_page_map_t256"]
+        _refused(ctx, ARG, "free", ctx.page_map, _cache(n_seqs=0), _map(rows=0, free_state=None, **kw))
+
+
 def test_a_rotation_is_first_used_outside_a_capture(ctx):
     ctx.capture_begin()
     with pytest.raises(hip.binding().G4aError, match="capture"):
