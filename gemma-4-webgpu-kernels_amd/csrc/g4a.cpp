@@ -2391,6 +2391,8 @@ int g4a_page_map(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_page_map_
     G4aPageMapParams p{};
     if (int rc = paged_cache(ctx, cache, true, false, &p.c)) return rc;
     if (!a) return fail(ctx, G4A_E_ARG, "null args");
+    // (the kernel's chunks of up to 1024 sequences and rows count past the last in 32 bits)
+    if (cache->n_seqs >> 31) return fail(ctx, G4A_E_SHAPE, "%u sequences: below 2^31", cache->n_seqs);
     if (a->rows >> 31) return fail(ctx, G4A_E_SHAPE, "%u rows: below 2^31", a->rows);
     if (a->rows_per_seq && uint64_t(a->rows_per_seq) * cache->n_seqs != a->rows)
         return fail(ctx, G4A_E_SHAPE, "%u rows are not %u for each of %u sequences", a->rows, a->rows_per_seq,

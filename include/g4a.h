@@ -538,7 +538,7 @@ typedef struct g4a_paged_cache {
  * free_cap must hold all pages that can be free at once. kv_len_out and
  * free_state_out receive the lengths and the state after the step, NULL:
  * cache->kv_len and free_state themselves; table and ring are written in place.
- * No two buffers of a call overlap otherwise.
+ * No two buffers of a call overlap otherwise. n_seqs is below 2^31.
  * The cache's pools and widths are not looked at. */
 typedef struct g4a_page_map_args {
     const uint32_t *new_len;      /* device [n_seqs], or NULL: one token each */

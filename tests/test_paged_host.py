@@ -130,6 +130,14 @@ def test_calls_past_a_launch_are_refused(ctx):
     _refused(ctx, SHAPE, "groups", ctx.kv_gather_paged, _cache(Dh=64), 0, 0, 16 * most + 1, PTR, PTR)
 
 
+def test_maps_of_more_sequences_than_are_counted_are_refused(ctx):
+    """The kernel counts sequences in 32 bits, up to 1024 past the last."""
+    ctx.page_map(_cache(n_seqs=(1 << 31) - 1, pages_per_seq=1), _map())
+    assert len(hip.launches()) == 1
+    for n in (1 << 31, 0xFFFFFC01, 0xFFFFFFFE):
+        _refused(ctx, SHAPE, "sequences", ctx.page_map, _cache(n_seqs=n, pages_per_seq=1), _map())
+
+
 def test_calls_without_work_launch_nothing(ctx):
     ctx.page_map(_cache(n_seqs=0), _map(rows=0))
     ctx.attn_producer_paged(_cache(), _producer(T=0))
