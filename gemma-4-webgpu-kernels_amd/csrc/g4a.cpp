@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -2327,6 +2328,10 @@ int g4a_attn_producer_devpos(g4a_ctx* ctx, const g4a_producer_args* a, const uin
 namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Words on the device, or null: the kernels take some of them by scalar loads, which drop an address's low bits.
+bool aligned4(std::initializer_list<const void*> ps) {
+    return std::all_of(ps.begin(), ps.end(), [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; });
+}
 
 // Fewest tiles (16 tokens) of a part of the paged decode: one for each wave.
 constexpr uint32_t PAGED_MIN_PART = 4;
@@ -2361,7 +2366,8 @@ int paged_cache(g4a_ctx* ctx, const g4a_paged_cache* c, bool tables, bool pools,
     *out = G4aPaged{c->k_pages, c->v_pages, c->block_table, c->kv_len, c->page_stride, c->n_seqs, c->pages_per_seq,
                     c->n_pages, uint32_t(__builtin_ctz(c->page_size)), c->Hkv, c->Dh, c->ring};
     if (tables && c->n_seqs) {
-        if (!c->block_table || !c->kv_len) return fail(ctx, G4A_E_ARG, "null block_table / kv_len");
+        if (!c->block_table || !c->kv_len || !aligned4({c->block_table, c->kv_len}))
+            return fail(ctx, G4A_E_ARG, "block_table / kv_len null or not 4-byte aligned");
         if (c->pages_per_seq == 0 || uint64_t(c->pages_per_seq) * c->page_size >= G4A_NO_ROW ||
             uint64_t(c->n_seqs) * c->pages_per_seq >= G4A_NO_ROW)
             return fail(ctx, G4A_E_SHAPE, "tables of %u x %u pages of %u tokens: a sequence's tokens and the table's "
@@ -2401,6 +2407,9 @@ int g4a_page_map(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_page_map_
     if (a->rows && (!a->slots || !a->positions)) return fail(ctx, G4A_E_ARG, "null slots / positions");
     if (!a->free_pages || !a->free_state || a->free_cap == 0)
         return fail(ctx, G4A_E_ARG, "null free_pages / free_state or an empty free ring");
+    if (!aligned4({a->new_len, a->shared_pages, a->free_pages, a->free_state, a->slots, a->positions, a->row_start,
+                   a->added, a->kv_len_out, a->free_state_out}))
+        return fail(ctx, G4A_E_ARG, "lengths, free ring, slots, positions and outputs must be 4-byte aligned");
     p.add = a->new_len;
     p.shared = a->shared_pages;
     p.free_pages = a->free_pages;
@@ -2437,6 +2446,7 @@ int g4a_attn_producer_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4
     if (a->T == 0) return G4A_OK;
     if (!a->q || !a->q_out || !a->positions || (a->k && !a->slots))
         return fail(ctx, G4A_E_ARG, "null q / q_out / positions / slots");
+    if (!aligned4({a->positions, a->slots})) return fail(ctx, G4A_E_ARG, "positions and slots must be 4-byte aligned");
     for (const void* x : {(const void*)a->q, (const void*)a->k, (const void*)a->v, (const void*)a->q_norm,
                           (const void*)a->k_norm, (const void*)a->q_out})
         if (!aligned16(x)) return fail(ctx, G4A_E_ARG, "rows and norm weights must be 16-byte aligned");

@@ -118,6 +118,25 @@ def test_bad_gathers_are_refused(ctx, code, text, args):
     _refused(ctx, code, text, ctx.kv_gather_paged, _cache(), *args)
 
 
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_words_off_their_four_bytes_are_refused(ctx, off):
+    """Tables, lengths, slots and positions are words at multiples of four bytes."""
+    for field in ("block_table", "kv_len"):
+        c = _cache(**{field: PTR + off})
+        _refused(ctx, ARG, "aligned", ctx.page_map, c, _map())
+        _refused(ctx, ARG, "aligned", ctx.attention_paged, c, _attn())
+        _refused(ctx, ARG, "aligned", ctx.kv_gather_paged, c, 0, 0, 5, PTR, PTR)
+        ctx.attn_producer_paged(c, _producer())  # which looks at the pools alone
+        assert len(hip.launches()) == 1
+    for field in ("new_len", "shared_pages", "free_pages", "free_state", "slots", "positions", "row_start", "added",
+                  "kv_len_out", "free_state_out"):
+        _refused(ctx, ARG, "aligned", ctx.page_map, _cache(), _map(**{field: PTR + off}))
+    for field in ("positions", "slots"):
+        _refused(ctx, ARG, "aligned", ctx.attn_producer_paged, _cache(), _producer(**{field: PTR + off}))
+    ctx.page_map(_cache(block_table=PTR + 4, kv_len=PTR + 8), _map(slots=PTR + 4, free_state=PTR + 12))
+    assert len(hip.launches()) == 1
+
+
 def test_calls_past_a_launch_are_refused(ctx):
     """A launch counts its threads in 32 bits: 2^24 - 1 workgroups of 256. At 512 dims a wave takes two rows of a
     token, four waves a workgroup; a gather of 64-dim rows takes a page of 16 a workgroup."""
