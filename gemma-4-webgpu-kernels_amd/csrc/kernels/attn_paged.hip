@@ -239,18 +239,12 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     if (each == 1) {
         len = __builtin_amdgcn_readlane(my_len, b);
     } else {
-        for (const uint32_t last = min(b + each, n);; b += 64) {
-            const uint32_t t = b + lane < last ? lane_parts(b + lane) : 0u;
-            const uint32_t u = wave_incl_sum(t);
-            const uint64_t hit = __ballot(base + u > at);
-            if (hit) {
-                const int l1 = __builtin_ctzll(hit);
-                base += __builtin_amdgcn_readlane(u - t, l1);
-                b += l1;
-                break;
-            }
-            base += __builtin_amdgcn_readlane(u, 63);
-        }
+        static_assert(PAGED_SEQS <= 64 * 64, "a lane's span of sequences, a lane each");
+        const uint32_t mine_of = lane < (int)min(each, n - b) ? lane_parts(b + lane) : 0u;
+        const uint32_t incl = wave_incl_sum(mine_of);
+        const int l1 = __builtin_ctzll(__ballot(base + incl > at));
+        base += __builtin_amdgcn_readlane(incl - mine_of, l1);
+        b += l1;
         len = __builtin_amdgcn_readfirstlane(lens[b]);
         barrier_lds();  // every wave has read the lengths: the query rows go there
     }
