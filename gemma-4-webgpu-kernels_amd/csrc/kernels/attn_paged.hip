@@ -179,6 +179,134 @@ __device__ __forceinline__ void pv_tile(f4v (&acc)[C::NA], const float (&pa)[C::
 typedef short bf4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4v __attribute__((ext_vector_type(4)));
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 0x1.fffffep127f; }
+
+// A wave's items of a part of bf16 pages once more, in f32 arithmetic on K and V as they are, where the products of
+// the three parts gave a value or a sum that is not finite: 0 times an infinity, or infinities of both signs, stand in
+// them where a token's K or V is infinite or a query is beyond bf16's largest value, and f32 products have neither.
+// Two passes over the part's tiles, the maxima and then the sums; s[q] is the score of head 4 q + lane / 16 and key
+// lane % 16, the items are those of the part's end. Heads whose sums were finite keep their maxima and sums, by which
+// the other waves' items go. Slow (8 sequences of up to 131072 keys of 512 dims: 131 us, with one infinity in V 2.7 ms,
+// with one in every page 3.6), and no cost where all is finite: such calls take what they took without it.
+template <typename C, int DH>
+__device__ __forceinline__ void paged_part_f32(const G4aPagedAttnParams& p, const PagedSpan& sp, uint32_t b, uint32_t kvh,
+                                               uint32_t h0, uint32_t nh, uint32_t from, uint32_t to, uint32_t at,
+                                               bool whole, int w, const float (*m_s)[C::HR], const float (*l_s)[C::HR]) {
+    constexpr int HR = C::HR, NQ = HR / 4, NI = (C::ITEMS + 255) / 256;
+    const G4aPaged& c = p.c;
+    // (the lane, and the divisor of page numbers, anew: nothing is kept for this over the tiles)
+    const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), id = 64 * w + ln;
+    const int g4 = ln >> 4, key = ln & 15;
+    uint32_t per_seq = c.per_seq;
+    asm volatile("" : "+s"(per_seq));
+    const size_t width = (size_t)c.Hkv * DH;
+    // each visible tile of the part: its first row in the pools, and its rows [lo, hi)
+    auto tiles = [&](auto&& use) {
+        for (uint32_t t = from; t < to; ++t) {
+            const uint32_t t0 = (sp.first + t) * 16, no = t0 >> c.page_shift;
+            const uint32_t page = load_scalar(c.table, (size_t)b * per_seq + (c.ring ? no % per_seq : no));
+            if (page >= c.n_pages) continue;
+            const uint32_t r = t0 & ((1u << c.page_shift) - 1);
+            use((size_t)page * c.page_stride + ((size_t)r * c.Hkv + kvh) * DH, sp.lo > t0 ? sp.lo - t0 : 0u,
+                min(16u, sp.len - t0));
+        }
+    };
+    auto scores = [&](f4v& s, size_t row, uint32_t lo, uint32_t hi) {
+        const u32x4* const k = reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(c.k) + row + key * width);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) s[q] = 0.0f;
+#pragma unroll 1
+        for (int d = 0; d < DH / 8; ++d) {
+            const u32x4 x = k[d];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                const float* const y = p.q + ((size_t)b * p.Hq + h0 + min((uint32_t)(4 * q + g4), nh - 1)) * DH + 8 * d;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    s[q] += __uint_as_float(e & 1 ? x[e / 2] & 0xFFFF0000u : x[e / 2] << 16) * y[e];
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            s[q] *= p.scale;
+            if (p.softcap > 0.0f) s[q] = p.softcap * tanhf(s[q] / p.softcap);
+            if ((uint32_t)key < lo || (uint32_t)key >= hi) s[q] = G4A_NEG_INF;
+        }
+    };
+    // (vectors: a choice among an array's elements became an index into scratch memory)
+    f4v m = {G4A_NEG_INF, G4A_NEG_INF, G4A_NEG_INF, G4A_NEG_INF}, l = {}, s, L_was = {};
+    tiles([&](size_t row, uint32_t lo, uint32_t hi) {
+        scores(s, row, lo, hi);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) m[q] = fmaxf(m[q], s[q]);
+    });
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        float M = G4A_NEG_INF;
+        for (int i = 0; i < 4; ++i) M = fmaxf(M, m_s[i][4 * q + g4]);
+        for (int i = 0; i < 4; ++i)
+            L_was[q] += l_s[i][4 * q + g4] * (m_s[i][4 * q + g4] == G4A_NEG_INF ? 0.0f : expf(m_s[i][4 * q + g4] - M));
+        m[q] = finite(L_was[q]) ? M : g4a_row_max16(m[q]);
+    }
+    f4v o[NI];
+#pragma unroll
+    for (int x = 0; x < NI; ++x) o[x] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    tiles([&](size_t row, uint32_t lo, uint32_t hi) {
+        scores(s, row, lo, hi);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            s[q] = s[q] == G4A_NEG_INF ? 0.0f : expf(s[q] - m[q]);
+            l[q] += s[q];
+        }
+#pragma unroll 1
+        for (uint32_t j = lo; j < hi; ++j)
+#pragma unroll
+            for (int x = 0; x < NI; ++x) {
+                const int i = id + 256 * x, hq = __builtin_amdgcn_readfirstlane(C::hq(i));  // (one for a wave's 64 items)
+                if (C::ITEMS < 256 && i >= C::ITEMS) continue;
+                const uint32_t v = reinterpret_cast<const uint16_t*>(c.v)[row + j * width + C::dim(i)];
+                float pw = s[0];
+#pragma unroll
+                for (int q = 1; q < NQ; ++q)
+                    if (hq == q) pw = s[q];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[x][r] += __shfl(pw, 16 * r + (int)j) * __uint_as_float(v << 16);
+            }
+    });
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) l[q] = finite(L_was[q]) ? L_was[q] : g4a_row_sum16(l[q]);
+    if (!whole && w == 0) {  // (the lanes that wrote these before)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const float M = __shfl(m[q], 16 * (ln & 3)), L = __shfl(l[q], 16 * (ln & 3));
+            if (ln / 4 == q) {
+                float* const ml = p.part_ml + (size_t)at * 2 * HR + ln;
+                ml[0] = M;
+                ml[HR] = L;
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < NI; ++x) {
+        const int i = id + 256 * x, hq = __builtin_amdgcn_readfirstlane(C::hq(i));
+        if (C::ITEMS < 256 && i >= C::ITEMS) continue;
+        if (!whole) {
+            (reinterpret_cast<f4v*>(p.part) + (size_t)at * C::ITEMS)[i] = o[x];
+            continue;
+        }
+        float L = l[0];
+#pragma unroll
+        for (int q = 1; q < NQ; ++q)
+            if (hq == q) L = l[q];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float sum = g4a_lane(L, 16 * r);
+            if (4 * hq + r < (int)nh)
+                p.out[((size_t)b * p.Hq + h0 + 4 * hq + r) * DH + C::dim(i)] = o[x][r] * (sum != 0.0f ? 1.0f / sum : 0.0f);
+        }
+    }
+}
+
 // WIN: a window's rows, which stay in the caches until the next step; a whole context's K and V
 // are read past them (16 ragged sequences 58.0 -> 55.3 us, eight of up to 131072 keys 163 -> 156;
 // 64 windows 31.7 us, read past the caches 32.8).
@@ -555,6 +683,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
         if (C::ML == 64 || ln < C::ML) mrg[(w * NA + d) * C::ML + ln] = acc[d];
     }
     const bool whole = parts == 1;
+    bool bad = false;  // bf16: a value that is not finite, or a sum
     if (id < HR) {
         float M = G4A_NEG_INF, L = 0.0f, f[4];
 #pragma unroll
@@ -564,6 +693,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
             f[i] = m_s[i][id] == G4A_NEG_INF ? 0.0f : expf(m_s[i][id] - M);
             L += l_s[i][id] * f[i];
         }
+        if constexpr (BF) bad = !finite(L);
         const float inv = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) f_s[i][id] = f[i] * inv;
@@ -590,6 +720,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
                 o += x * f;
             }
         }
+        if constexpr (BF) bad |= !(finite(o[0]) && finite(o[1]) && finite(o[2]) && finite(o[3]));
         if (whole) {
             const int dim = C::dim(i);
 #pragma unroll
@@ -599,6 +730,8 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
             dst[i] = o;
         }
     }
+    if constexpr (BF)
+        if (__ballot(bad)) paged_part_f32<C, DH>(p, sp, b, kvh, h0, nh, s, e, at, whole, w, m_s, l_s);
 }
 
 // Merges the partials of units that more than one workgroup worked on. A block of W waves takes CI items (4 heads, one

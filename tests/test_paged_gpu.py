@@ -220,6 +220,67 @@ def test_attention_shows_infinities_and_nan_of_visible_tokens_only(ctx):
     c.free()
 
 
+def _same(got, want, bound, what):
+    """Infinities and NaN where the definition has them, the rest within the bound."""
+    got, rest = got.astype(np.float64), np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    assert np.array_equal(got[~rest & ~np.isnan(want)], want[~rest & ~np.isnan(want)]), what
+    _close(got[rest], want[rest], bound[rest], what)
+
+
+@pytest.mark.parametrize("kv_type", ["f32", "bf16"])
+@pytest.mark.parametrize("dh,hq,hkv", [(64, 4, 1), (64, 8, 1), (64, 16, 1), (128, 3, 1), (128, 16, 2), (128, 12, 1),
+                                       (256, 4, 1), (256, 8, 1), (256, 20, 1), (512, 2, 1), (512, 16, 2), (512, 9, 1)])
+def test_attention_of_infinite_values(ctx, dh, hq, hkv, kv_type):
+    """Visible infinities and NaN act as in f32 arithmetic whatever the pages hold, in sequences of one part and of
+    many: V's reach their dim of their kv head's output; a key of minus infinity has weight 0 where a query's value
+    there is positive, and makes the row NaN where it is negative; a query's value near f32's largest times a key's
+    near its smallest is a score like any other."""
+    say(f"infinite values: dh {dh} heads {hq}/{hkv} {kv_type}")
+    opts = dict(dh=dh, hkv=hkv, kv_type=kv_type, unit=0.05 * np.sqrt(256 / dh), seed=dh + hq)
+    c = Paged(ctx, [50, 700, 17, 0], **opts)
+    q = c.queries(hq)
+
+    def attend(q=q):
+        for d, x in zip(c.dev, (c.k, c.v)):
+            ctx.h2d(d.ptr, ref.pack(x, kv_type))
+        return c.attend(q)
+
+    plain = [c.want(q), c.k.copy(), c.v.copy()]
+    for b, e in ((0, 1), (1, 20), (2, 0)):  # V, infinite and NaN
+        c.v[c.table[b, e], 3, hkv - 1, 17] = np.inf
+        c.v[c.table[b, e], 5, 0, dh - 1] = -np.inf
+        c.v[c.table[b, e], 7, 0, 2] = np.nan
+    c.v[c.table[1, 30], 1, hkv - 1, 17] = -np.inf
+    with np.errstate(all="ignore"):
+        want, bound = c.want(q)
+    assert np.isnan(want).any() and np.isposinf(want).any() and np.isneginf(want).any()
+    _same(attend(), want, bound, "V")
+
+    c.k, c.v = plain[1].copy(), plain[2].copy()
+    pages = [c.table[0, 1], c.table[1, 20]]  # K of whole pages: as if they were not there, for a query positive there
+    c.k[pages, :, :, 33] = -np.inf
+    got = attend()
+    held = c.table.copy()
+    c.table[0, 1] = c.table[1, 20] = ref.NO_ROW
+    want, bound = (x.reshape(4, hq, dh).copy() for x in c.want(q))
+    c.table = held
+    want[:2][q[:2, :, 33] < 0] = np.nan
+    _same(got.reshape(want.shape), want, bound, "K")
+
+    # products as of 2^-120 of the query's value and 2^120 of the key's, which the bound is taken of
+    c.k, c.v = plain[1].copy(), plain[2].copy()
+    far, far_q, live = c.k.copy(), q.copy(), np.isfinite(c.k[..., 5])
+    c.k[..., 5][live], far[..., 5][live] = 2.0 ** -6, 2.0 ** -126
+    far_q[:, :, 5] = np.where(q[:, :, 5] > 0, 3.4e38, -3.4e38)
+    q2 = far_q.copy()
+    q2[:, :, 5] *= 2.0 ** -120
+    want, bound = c.want(q2)
+    c.k = far
+    _same(attend(far_q), want, bound, "the query")
+    c.free()
+
+
 def test_attention_is_repeatable_and_shares_pages(ctx):
     """Two sequences over the same pages, twice: the same bits."""
     c = Paged(ctx, [3000, 3000, 17], dh=512, page=32, seed=7)
