@@ -2339,14 +2339,18 @@ constexpr uint32_t PAGED_MIN_PART = 4;
 constexpr uint32_t PAGED_MAX_PARTS = 1024;
 // Most sequences of a launch (attn_paged.hip).
 constexpr uint32_t PAGED_SEQS = 1024;
-// Units up to which a merge block takes 16 items of one, not 64.
+// Units up to which a merge block takes 16 items of one, not 64. (Sequences of up to 8192 tokens of 512 dims, a call
+// with 16 and with 64: 1 unit 32.3 us (32768 tokens) and 37.2, 2 18.7 and 21.3, 4 20.4 and 22.8, 8 26.5 and 27.7;
+// 12 34.7 and 36.0, 16 40.0 and 40.4, 24 56.8 and 55.6, 32 72.3 and 69.3. Windows of 512 tokens of 256 dims are within
+// 5 % either way up to 16 units, 32 16.5 and 16.4, 64 24.5 and 21.1.)
 constexpr uint32_t PAGED_FEW_UNITS = 8;
 // Most workgroups of 256 threads of a launch: their threads along x are counted in 32 bits.
 constexpr uint32_t PAGED_GRID = 0xFFFFFF;
 // Most units of a launch (but for a sequence that has more).
 constexpr uint32_t PAGED_UNITS = 2048;
-// Its workgroups per CU (at 512 dims and up to 8 heads there is room for two, but a call of a few parts a
-// unit is faster with one: 16 ragged sequences of f32 pages 40.9 us, 49.0):
+// Its workgroups per CU (at 512 dims and up to 8 heads there is room for two, but most calls are faster with one:
+// 16 ragged sequences of f32 pages 40.4 us and 44.5, 256 of up to 1500 tokens 114 and 143, but 100 of up to 4000
+// 125 and 105):
 // [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
 constexpr uint32_t PAGED_WGS_PER_CU[4][2][3] = {
     {{4, 4, 2}, {4, 4, 4}}, {{3, 3, 2}, {4, 4, 3}}, {{2, 2, 1}, {3, 3, 2}}, {{1, 1, 1}, {1, 1, 1}}};
@@ -2451,8 +2455,8 @@ int g4a_attn_producer_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4
                           (const void*)a->k_norm, (const void*)a->q_out})
         if (!aligned16(x)) return fail(ctx, G4A_E_ARG, "rows and norm weights must be 16-byte aligned");
     // More rows of a token to a wave share its sines and their loads overlap, but fewer waves run
-    // at once (4099 tokens of 10 rows of 256: 21.8, 18.3, 18.2 us with 1, 2, 5 turns a wave; 16384:
-    // 88.8, 73.0, 64.6, and 67.2 with 4; 512: 4.9, 5.2, 6.6). A row of 512 is two loads a lane already.
+    // at once (4099 tokens of 10 rows of 256: 19.3, 16.9, 16.5, 16.8 us with 1, 2, 4, 5 turns a wave; 16384:
+    // 86.8, 68.6, 64.6, 63.2; 512: 5.2, 5.4, 6.1, 6.4). A row of 512 is two loads a lane already.
     const uint32_t at_once = std::max<uint32_t>(1, 256 / cache->Dh);  // rows a wave holds
     const uint32_t cus = uint32_t(std::max(ctx->cu_count, 1));
     const uint32_t turns = a->T < 4 * cus ? 1 : a->T < 32 * cus || cache->Dh > 256 ? 2 : 4;
@@ -2510,15 +2514,17 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     const int d = paged_dh(cache->Dh), t = int(cache->kv_type);
     const uint32_t resident = uint32_t(std::max(ctx->cu_count, 1)) * PAGED_WGS_PER_CU[d][t][h];
     // Parts to aim at where there are many units: at 512 dims and up to 8 heads half as many more, which the
-    // second workgroup that a CU has room for takes (256 sequences of up to 1500 tokens, f32: 115 us with them,
-    // 145 without, 129 with as many again; 100 of up to 4000, where there are fewer units, are not concerned).
+    // second workgroup that a CU has room for takes (256 sequences of up to 1500 tokens, f32: 114 us with them,
+    // 143 without, 127 with as many again; bf16 69, 82, 79; 100 of up to 4000, where there are fewer units, are not
+    // concerned).
     const uint32_t over = d == 3 && h < 2 ? resident + resident / 2 : resident;
     // launches of at most PAGED_UNITS units, which bounds the partials' memory, and of as many sequences as
     // the kernel counts
     const uint32_t most = std::min({cache->n_seqs, std::max(1u, PAGED_UNITS / p.units), PAGED_SEQS});
     // Parts: `resident` and no more where that is a few parts a unit, and else about one a unit more, which
-    // leaves as the others end. (One or two workgroups a CU: 96 sequences of 512 dims 38.8 us, 57.1 beyond
-    // what runs at once; four a CU: 512 units of 128 dims 48.6, 42.4.)
+    // leaves as the others end. (A few is two where one or two workgroups run a CU, and three beyond: 96 sequences of
+    // up to 1500 tokens of 512 dims take 47.4 us with two, 53.5 with three; 512 units of 128 dims in bf16 pages, four
+    // workgroups a CU, 41.4 with three, 49.9 with two.)
     auto shares = [&](uint32_t seqs, uint32_t* spread, uint32_t* fit) {
         const uint64_t units = uint64_t(seqs) * p.units, tiles = uint64_t(p.span / 16 + 2) * units;
         const uint64_t most_parts = std::min<uint64_t>(std::min(resident, PAGED_MAX_PARTS), tiles / PAGED_MIN_PART + units);

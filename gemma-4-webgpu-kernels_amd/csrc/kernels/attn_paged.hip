@@ -12,8 +12,9 @@
 // part from the lengths itself. A part that is its whole unit writes the output, any
 // other a partial (O, m, l), which paged_combine merges. (Equal runs of tiles across
 // units, with the next unit's first tile loaded behind the last of the one before,
-// balanced better and were slower: 16 ragged sequences 52.0 against 48.3 us, 128 of 4 kv
-// heads 68.2 against 55.8: several merges a workgroup, and 40 more registers.)
+// balanced better and were slower in an early form: 16 ragged sequences 52.0 against
+// 48.3 us, 128 of 4 kv heads 68.2 against 55.8: several merges a workgroup, and 40 more
+// registers.)
 //
 // A workgroup is 4 waves, each on every fourth tile of its part, with K and V of
 // the next tile in flight in registers (16-byte loads; no LDS in between):
@@ -308,8 +309,9 @@ __device__ __forceinline__ void paged_part_f32(const G4aPagedAttnParams& p, cons
 }
 
 // WIN: a window's rows, which stay in the caches until the next step; a whole context's K and V
-// are read past them (16 ragged sequences 58.0 -> 55.3 us, eight of up to 131072 keys 163 -> 156;
-// 64 windows 31.7 us, read past the caches 32.8).
+// are read past them (the other way about: 16 ragged sequences 42.2 us for 40.4, eight of up to 131072 keys 142 for
+// 131, 128 of 4 kv heads 45.3 for 41.8, 64 windows 18.3 for 17.0, in f32 pages 23.0 for 21.1; only one sequence of
+// 32768 keys, read again and again, gains: 31.6 for 32.5).
 template <int DH, typename KV, int NHQ, bool WIN>
 __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     using C = PagedCfg<DH, KV, NHQ>;
@@ -404,9 +406,9 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     };
     // 512 dims: K and V take turns in one set of registers, V's pieces loaded where K's have been used and
     // K's next where V's have. With 16 heads there is no room for both; with up to 8 a second workgroup of a
-    // CU starts while the first ends (256 ragged sequences of up to 1500 tokens in bf16 pages: 69.7 us, and
-    // 83.6 with both in flight; one of 32768 in f32 pages 32.6 and 34.5; but eight of up to 131072 in bf16
-    // pages 132.4 and 131.3).
+    // CU starts while the first ends (256 ragged sequences of up to 1500 tokens in bf16 pages: 68.7 us, and
+    // 78.3 with both in flight; one of 32768 in f32 pages 32.4 and 34.6; eight of up to 131072 in bf16 pages
+    // 131.2 and 130.4, which runs differ by as well).
     constexpr bool TURNS = DH == 512;
     VWord v[C::VL];  // bf16: [row][block of dims]
     u32x4 k_own[TURNS ? 1 : KC];
@@ -736,9 +738,9 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
 
 // Merges the partials of units that more than one workgroup worked on. A block of W waves takes CI items (4 heads, one
 // dim) of a unit, 64 W / CI groups of threads every such part of it: 16 items and 8
-// waves where there are few units of many parts (256 parts of 512 dims: with 64 items
-// and 4 waves a call took 36.9 us, 32.5 so; a window of 512 on 4, 8, 16 waves 11.1, 11.2,
-// 11.6), 64 items and 4 waves where there are many units. A thread's first partial is loaded with the parts' maxima
+// waves where there are few units of many parts (one unit of 256 parts of 512 dims: with
+// 64 items and 4 waves a call takes 37.2 us, 32.2 so), 64 items and 4 waves where there are many units (64 of
+// up to 4000 tokens 72.1 us, 79.0 with 16). A thread's first partial is loaded with the parts' maxima
 // and sums, ahead of the weights e^(m - M), which are computed a part a thread and meet
 // in LDS.
 constexpr int PAGED_PARTS = 1024;  // of a unit, at most

@@ -72,8 +72,11 @@ __device__ __forceinline__ uint32_t last_at_or_before(const uint32_t* start, uin
 // its share of each chunk's rows: the scans are a microsecond of latency, less than a
 // second launch. Lengths and ring state are written by workgroup 0 where they have
 // buffers of their own, else by the workgroup that draws the last ticket, which is
-// after every other's reads of them. 64 sequences of one token: 4.8 us with 64-bit sums,
-// shuffles and a third scan for rows refused, which only a chunk that refuses some needs.
+// after every other's reads of them, in a second pass over the sequences: 512 of them and
+// 65536 rows take 10.3 us in place, 6.4 with buffers of their own, 64 of one token (one
+// workgroup, one pass) 4.3 and 3.8. The sums are 32 bits wide and their third scan is for
+// chunks that refuse rows alone (64 sequences of one token 4.1 us a call; 4.8 with 64-bit
+// sums, shuffles and three scans each).
 template <int T>
 __device__ __forceinline__ void page_map(const G4aPageMapParams& p) {
     __shared__ uint32_t s_start[T], s_len[T], s_had[T], s_base[T], s_added[T], s_rel[T], s_keep[T];
@@ -224,8 +227,8 @@ __device__ __forceinline__ void store4(__bf16* p, const f32x4& v) {
 //
 // A row takes DH / 4 lanes (two float4 each at 512), so a wave holds 256 / DH of them at a
 // time; it takes heads_per_wave rows of one token, the next rows' loads ahead of the work
-// on these. Bound by HBM in long calls: 16384 tokens of 10 rows of 256 take 67 us (5.0
-// TB/s read and written) with four turns a wave, 89 with one; one token 3.3 us and 5.2.
+// on these. Bound by HBM in long calls: 16384 tokens of 10 rows of 256 take 65 us (5.2
+// TB/s read and written) with four turns a wave, 87 with one; one token 5.1 us and 3.9.
 constexpr int PP_WAVES = 4;
 
 template <int DH, typename KV>
