@@ -182,6 +182,30 @@ typedef __bf16 bf16x4v __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 0x1.fffffep127f; }
 
+// The heads of a unit whose query holds a NaN: their output is NaN in any arithmetic, so paged_part_f32 is not called
+// for them (a sequence that pauses may have anything in its row of q; 8 sequences of up to 131072 keys of 512 dims with
+// NaN in every query 138 us, with it 4.2 ms).
+template <typename C, int DH>
+__device__ __forceinline__ uint32_t nan_queries(const G4aPagedAttnParams& p, uint32_t b, uint32_t h0, uint32_t nh) {
+    const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    uint32_t heads = 0;
+#pragma unroll
+    for (int q = 0; q < C::HR / 4; ++q) {
+        const uint32_t h = h0 + min((uint32_t)(4 * q + ln / 16), nh - 1);
+        const f4v* const y = reinterpret_cast<const f4v*>(p.q + ((size_t)b * p.Hq + h) * DH);
+        bool is = false;
+#pragma unroll
+        for (int d = 0; d < DH / 64; ++d) {
+            const f4v x = y[ln % 16 + 16 * d];
+            is |= x[0] != x[0] || x[1] != x[1] || x[2] != x[2] || x[3] != x[3];
+        }
+        const uint64_t lanes = __ballot(is);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) heads |= (lanes >> (16 * g) & 0xFFFF ? 1u : 0u) << (4 * q + g);
+    }
+    return heads;
+}
+
 // A wave's items of a part of bf16 pages once more, in f32 arithmetic on K and V as they are, where the products of
 // the three parts gave a value or a sum that is not finite: 0 times an infinity, or infinities of both signs, stand in
 // them where a token's K or V is infinite or a query is beyond bf16's largest value, and f32 products have neither.
@@ -685,7 +709,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
         if (C::ML == 64 || ln < C::ML) mrg[(w * NA + d) * C::ML + ln] = acc[d];
     }
     const bool whole = parts == 1;
-    bool bad = false;  // bf16: a value that is not finite, or a sum
+    bool sum_bad = false;
     if (id < HR) {
         float M = G4A_NEG_INF, L = 0.0f, f[4];
 #pragma unroll
@@ -695,7 +719,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
             f[i] = m_s[i][id] == G4A_NEG_INF ? 0.0f : expf(m_s[i][id] - M);
             L += l_s[i][id] * f[i];
         }
-        if constexpr (BF) bad = !finite(L);
+        sum_bad = !finite(L);
         const float inv = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) f_s[i][id] = f[i] * inv;
@@ -705,6 +729,7 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
             ml[HR] = L;
         }
     }
+    uint32_t bad = BF ? (uint32_t)__ballot(sum_bad) : 0u;  // heads with a sum or a value that is not finite
     barrier_lds();
     f4v* const dst = reinterpret_cast<f4v*>(p.part) + (size_t)at * C::ITEMS;
     for (int i = id; i < C::ITEMS; i += 256) {
@@ -722,7 +747,10 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
                 o += x * f;
             }
         }
-        if constexpr (BF) bad |= !(finite(o[0]) && finite(o[1]) && finite(o[2]) && finite(o[3]));
+        if constexpr (BF)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                bad |= (__ballot(!finite(o[r])) ? 1u : 0u) << (4 * __builtin_amdgcn_readfirstlane(hq) + r);
         if (whole) {
             const int dim = C::dim(i);
 #pragma unroll
@@ -732,8 +760,11 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
             dst[i] = o;
         }
     }
-    if constexpr (BF)
-        if (__ballot(bad)) paged_part_f32<C, DH>(p, sp, b, kvh, h0, nh, s, e, at, whole, w, m_s, l_s);
+    if constexpr (BF) {
+        bad &= (1u << nh) - 1;
+        if (bad && (bad & ~nan_queries<C, DH>(p, b, h0, nh)))
+            paged_part_f32<C, DH>(p, sp, b, kvh, h0, nh, s, e, at, whole, w, m_s, l_s);
+    }
 }
 
 // Merges the partials of units that more than one workgroup worked on. A block of W waves takes CI items (4 heads, one

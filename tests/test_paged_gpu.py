@@ -281,6 +281,25 @@ def test_attention_of_infinite_values(ctx, dh, hq, hkv, kv_type):
     c.free()
 
 
+@pytest.mark.parametrize("kv_type", ["f32", "bf16"])
+@pytest.mark.parametrize("dh,hq,hkv", [(64, 16, 1), (128, 3, 1), (256, 8, 1), (512, 9, 1)])
+def test_attention_of_queries_that_are_nan(ctx, dh, hq, hkv, kv_type):
+    """A NaN in a query makes its head's row NaN and no other's, beside an infinity in V or not."""
+    say(f"NaN queries: dh {dh} heads {hq}/{hkv} {kv_type}")
+    c = Paged(ctx, [50, 700, 17, 90], dh=dh, hkv=hkv, kv_type=kv_type, seed=dh)
+    q = c.queries(hq)
+    q[1, 0, dh - 1] = q[2, :, 40] = q[3, hq - 1, 3] = np.nan
+    for poison in (False, True):
+        if poison:
+            c.v[c.table[1, 20], 3, 0, 17] = c.v[c.table[3, 1], 2, 0, 5] = -np.inf
+            ctx.h2d(c.dev[1].ptr, ref.pack(c.v, kv_type))
+        with np.errstate(all="ignore"):
+            want, bound = c.want(q)
+        assert np.isnan(want.reshape(4, hq, dh)).all(-1).sum() == 1 + hq + 1 and np.isinf(want).any() == poison
+        _same(c.attend(q), want, bound, f"NaN queries, infinities {poison}")
+    c.free()
+
+
 def test_attention_is_repeatable_and_shares_pages(ctx):
     """Two sequences over the same pages, twice: the same bits."""
     c = Paged(ctx, [3000, 3000, 17], dh=512, page=32, seed=7)
