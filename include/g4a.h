@@ -527,9 +527,10 @@ typedef struct g4a_paged_cache {
  * G4A_NO_ROW; so does the slot of a token that a ring loses within the step.
  *
  * A sequence adds all of its tokens or none. None: if they do not fit its table
- * (linear), 2^32 - 2 tokens in all (a ring) or rows_per_seq, if it needs pages and the running sum of the pages
- * needed so far, in sequence order, passes the free ones, or, packed, if the
- * running sum of rows passes `rows`. added[b] says how many it got. A sequence of
+ * (linear), 2^32 - 2 tokens in all (a ring) or rows_per_seq, if it needs pages and
+ * the running sum of the pages needed so far, in sequence order, passes the free
+ * ones, or, packed, if the running sum of rows passes `rows`. added[b] says how
+ * many it got. A sequence of
  * new_len G4A_SEQ_END ends: its pages, but for the first shared_pages[b], go to
  * the end of the free ring in table order (for the next call) and its length
  * becomes 0. Its entries go there as they stand, also one that names no page: of
@@ -590,8 +591,9 @@ int g4a_attn_producer_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4
  * soft-cap as in g4a_attention; zeros where kv_len[b] is 0. Lengths alone say
  * what is attended: a sequence that got no token this step (added[b] is 0) is read
  * and its output row written all the same, from whatever its row of q holds, for
- * the caller to pass over. Query head h reads kv head h / (Hq / Hkv). Every kernel and grid depends on the arguments alone, so a
- * captured call follows lengths and tables. The partial results of sequences that
+ * the caller to pass over. Query head h reads kv head h / (Hq / Hkv). Every kernel
+ * and grid depends on the arguments alone, so a captured call follows lengths and
+ * tables. The partial results of sequences that
  * several workgroups share stand in the context's workspace: run the call once, at
  * its sizes, before capturing it. Results are the same bits from call to call. */
 typedef struct g4a_paged_attn_args {
