@@ -152,12 +152,14 @@ struct g4a_ctx {
     hipFunction_t slice_cols = nullptr;
     hipFunction_t rms_rows = nullptr;        // (residual +) RMSNorm (* scalar) over rows of any width
     hipFunction_t embed_f32 = nullptr;
-    // the paged KV cache: [head_dim 64, 128, 256, 512][f32, bf16 pages]
+    // the paged KV cache: [head_dim 64, 128, 256, 512][f32, bf16, 8-bit, 4-bit pages]
     hipFunction_t page_map[2] = {};  // [256, 1024 threads]
-    hipFunction_t paged_producer[4][2] = {};
-    hipFunction_t paged_decode[2][4][2][3] = {};  // [whole context, window] ... [4, 8, 16 heads a unit]
-    hipFunction_t paged_combine[2][4][2][3] = {};  // [16, 64 items a block] ...
-    hipFunction_t paged_gather[2] = {};
+    hipFunction_t paged_producer[4][4] = {};
+    hipFunction_t paged_decode[2][4][4][3] = {};  // [whole context, window] ... [4, 8, 16 heads a unit]
+    hipFunction_t paged_combine[2][4][4][3] = {};  // [16, 64 items a block] ...
+    hipFunction_t paged_gather[2] = {};            // f32 and bf16 pages, any head_dim
+    hipFunction_t paged_write[4][4] = {};
+    hipFunction_t paged_read[4][4] = {};
     uint32_t* ticket = nullptr;  // g4a_page_map's: 0 between launches
     // RoPE frequency tables theta^(-2j/rot), one per (theta, rotary_dim) seen
     struct FreqTable {
@@ -182,7 +184,7 @@ struct g4a_ctx {
     hipEvent_t ev_staging = nullptr;  // last use of the pinned staging buffer
     void* workspace = nullptr;
     size_t workspace_bytes = 0;
-    int query_depth = 0;              // > 0 inside a query entry point (g4a_attention_plan)
+    int query_depth = 0;              // > 0 inside a query entry point (g4a_attention_plan, g4a_kv_page_bytes)
     void* scratch = nullptr;  // this device's static scratch array (the allocation-free entry point)
     hipFunction_t prefill_merge[2] = {nullptr, nullptr};  // [dh512] merge of split prefill blocks
     float* dummy = nullptr;  // 4 KiB of zeros: the load target of idle decode tiles
@@ -594,6 +596,13 @@ int launch(g4a_ctx* ctx, hipFunction_t f, dim3 grid, dim3 block, const P& params
     return G4A_OK;
 }
 
+// In a query: its failures do not discard an open graph capture.
+struct QueryScope {
+    g4a_ctx* c;
+    explicit QueryScope(g4a_ctx* x) : c(x) { if (c) ++c->query_depth; }
+    ~QueryScope() { if (c) --c->query_depth; }
+};
+
 // Host-side analysis shared by g4a_attention and g4a_attention_plan.
 struct Analysis {
     g4a_attn_plan plan{};
@@ -909,25 +918,34 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
     }
     if (int rc = get_fn(ctx, &ctx->page_map[0], "g4a_page_map_t256")) return bail(rc);
     if (int rc = get_fn(ctx, &ctx->page_map[1], "g4a_page_map_t1024")) return bail(rc);
-    for (int t = 0; t < 2; ++t) {
-        const char* const type = t ? "bf16" : "f32";
+    for (int t = 0; t < 4; ++t) {
+        static const char* const types[4] = {"f32", "bf16", "i8", "i4"};
         char name[64];
         for (int d = 0; d < 4; ++d) {
-            snprintf(name, sizeof name, "g4a_paged_producer_d%d_%s", 64 << d, type);
-            if (int rc = get_fn(ctx, &ctx->paged_producer[d][t], name)) return bail(rc);
+            struct Row {
+                hipFunction_t* fn;
+                const char* what;
+            };
+            for (const Row& r : {Row{&ctx->paged_producer[d][t], "producer"}, Row{&ctx->paged_write[d][t], "write"},
+                                 Row{&ctx->paged_read[d][t], "read"}}) {
+                snprintf(name, sizeof name, "g4a_paged_%s_d%d_%s", r.what, 64 << d, types[t]);
+                if (int rc = get_fn(ctx, r.fn, name)) return bail(rc);
+            }
             for (int h = 0; h < 3; ++h) {
                 for (int win = 0; win < 2; ++win) {
-                    snprintf(name, sizeof name, "g4a_paged_decode%s_d%d_%s_h%d", win ? "_win" : "", 64 << d, type, 1 << h);
+                    snprintf(name, sizeof name, "g4a_paged_decode%s_d%d_%s_h%d", win && t < 2 ? "_win" : "", 64 << d, types[t],
+                             1 << h);
                     if (int rc = get_fn(ctx, &ctx->paged_decode[win][d][t][h], name)) return bail(rc);
                 }
                 for (int w = 0; w < 2; ++w) {
-                    snprintf(name, sizeof name, "g4a_paged_combine%d_d%d_%s_h%d", w ? 64 : 16, 64 << d, type, 1 << h);
+                    snprintf(name, sizeof name, "g4a_paged_combine%d_d%d_%s_h%d", w ? 64 : 16, 64 << d, types[t], 1 << h);
                     if (int rc = get_fn(ctx, &ctx->paged_combine[w][d][t][h], name)) return bail(rc);
                 }
             }
         }
-        snprintf(name, sizeof name, "g4a_paged_gather_%s", type);
-        if (int rc = get_fn(ctx, &ctx->paged_gather[t], name)) return bail(rc);
+        snprintf(name, sizeof name, "g4a_paged_gather_%s", types[t]);
+        if (t < 2)
+            if (int rc = get_fn(ctx, &ctx->paged_gather[t], name)) return bail(rc);
     }
     if (hipMalloc(reinterpret_cast<void**>(&ctx->dummy), 4096) != hipSuccess ||
         hipMemset(ctx->dummy, 0, 4096) != hipSuccess) {
@@ -1044,12 +1062,7 @@ int g4a_stream(g4a_ctx* ctx, void** stream) {
 }
 
 int g4a_attention_plan(g4a_ctx* ctx, const g4a_attn_args* a, g4a_attn_plan* plan) {
-    // a query: its failures do not discard an open graph capture
-    struct Query {
-        g4a_ctx* c;
-        explicit Query(g4a_ctx* x) : c(x) { if (c) ++c->query_depth; }
-        ~Query() { if (c) --c->query_depth; }
-    } q(ctx);
+    QueryScope q(ctx);
     if (!plan) return fail(ctx, G4A_E_ARG, "null plan");
     Analysis an;
     if (int rc = analyse(ctx, a, &an, false)) return rc;
@@ -2351,12 +2364,28 @@ constexpr uint32_t PAGED_UNITS = 2048;
 // Its workgroups per CU (at 512 dims and up to 8 heads there is room for two, but most calls are faster with one:
 // 16 ragged sequences of f32 pages 40.4 us and 44.5, 256 of up to 1500 tokens 114 and 143, but 100 of up to 4000
 // 125 and 105):
-// [head_dim 64, 128, 256, 512][f32, bf16 pages][4, 8, 16 heads a unit].
-constexpr uint32_t PAGED_WGS_PER_CU[4][2][3] = {
-    {{4, 4, 2}, {4, 4, 4}}, {{3, 3, 2}, {4, 4, 3}}, {{2, 2, 1}, {3, 3, 2}}, {{1, 1, 1}, {1, 1, 1}}};
+// [head_dim 64, 128, 256, 512][f32, bf16, 8-bit, 4-bit pages][4, 8, 16 heads a unit].
+constexpr uint32_t PAGED_WGS_PER_CU[4][4][3] = {
+    {{4, 4, 2}, {4, 4, 4}, {4, 4, 4}, {4, 4, 4}},
+    {{3, 3, 2}, {4, 4, 3}, {4, 4, 3}, {4, 4, 3}},
+    {{2, 2, 1}, {3, 3, 2}, {3, 3, 2}, {3, 3, 2}},
+    {{1, 1, 1}, {1, 1, 1}, {1, 1, 1}, {1, 1, 1}}};
 
 // Index of a paged cache's head_dim among the kernels'.
 int paged_dh(uint32_t Dh) { return Dh == 64 ? 0 : Dh == 128 ? 1 : Dh == 256 ? 2 : 3; }
+// Index of its kv_type, -1: none.
+int paged_type(uint32_t kv_type) {
+    return kv_type == G4A_KV_F32 ? 0 : kv_type == G4A_KV_BF16 ? 1 : kv_type == G4A_KV_I8 ? 2 : kv_type == G4A_KV_I4 ? 3 : -1;
+}
+// Pages of 8 and 4 bits: their page_stride counts bytes, their rows are as paged_quant.h says.
+bool paged_quant(uint32_t kv_type) { return kv_type == G4A_KV_I8 || kv_type == G4A_KV_I4; }
+// Units (values; bytes of pages of 8 and 4 bits) of a page.
+uint64_t paged_page(const g4a_paged_cache* c) {
+    const uint64_t rows = uint64_t(c->page_size) * c->Hkv;
+    if (!paged_quant(c->kv_type)) return rows * c->Dh;
+    const uint64_t subs = c->kv_type == G4A_KV_I4 ? c->Dh / 32 : 0;
+    return (rows * (uint64_t(c->Dh) * c->kv_type / 8 + subs + 2) + 127) / 128 * 128;
+}
 
 // Checks a paged cache's tables (`tables`) and pools and widths (`pools`), and gives
 // the kernels' form of it.
@@ -2381,17 +2410,30 @@ int paged_cache(g4a_ctx* ctx, const g4a_paged_cache* c, bool tables, bool pools,
         if (c->Dh != 64 && c->Dh != 128 && c->Dh != 256 && c->Dh != 512)
             return fail(ctx, G4A_E_UNSUPPORTED, "head_dim %u: paged caches have 64, 128, 256 or 512", c->Dh);
         if (c->Hkv == 0 || c->Hkv > 1024) return fail(ctx, G4A_E_UNSUPPORTED, "Hkv %u is not 1 .. 1024", c->Hkv);
-        if (c->kv_type != G4A_KV_F32 && c->kv_type != G4A_KV_BF16)
+        if (paged_type(c->kv_type) < 0)
             return fail(ctx, G4A_E_ARG, "kv_type %u is no g4a_kv_type", c->kv_type);
         if (!c->k_pages || !c->v_pages || !aligned16(c->k_pages) || !aligned16(c->v_pages))
             return fail(ctx, G4A_E_ARG, "k_pages / v_pages null or not 16-byte aligned");
-        const uint64_t page = uint64_t(c->page_size) * c->Hkv * c->Dh;
-        if (c->page_stride && (c->page_stride % 8 || c->page_stride < page || c->page_stride >> 40))
-            return fail(ctx, G4A_E_SHAPE, "page_stride %llu: a multiple of 8 values from the page's %llu on, below 2^40",
-                        (unsigned long long)c->page_stride, (unsigned long long)page);
+        const uint64_t page = paged_page(c);
+        const bool quant = paged_quant(c->kv_type);
+        if (c->page_stride && (c->page_stride % (quant ? 16 : 8) || c->page_stride < page || c->page_stride >> 40))
+            return fail(ctx, G4A_E_SHAPE, "page_stride %llu: a multiple of %s from the page's %llu on, below 2^40",
+                        (unsigned long long)c->page_stride, quant ? "16 bytes" : "8 values", (unsigned long long)page);
         if (!c->page_stride) out->page_stride = page;
     }
     return G4A_OK;
+}
+
+// Launches a kernel on T * Hkv rows of K and as many of V: a wave takes `turns` lots of them, one after the other.
+int paged_rows(g4a_ctx* ctx, const g4a_paged_cache* c, hipFunction_t (&kernels)[4][4], G4aPagedRowsParams& p,
+               const char* what) {
+    const uint32_t at_once = std::max<uint32_t>(1, 256 / c->Dh);  // rows a wave holds
+    const uint64_t rows = uint64_t(p.T) * c->Hkv;
+    p.turns = 1;
+    const uint64_t wgs = (rows + 4 * p.turns * at_once - 1) / (4 * p.turns * at_once);
+    if (wgs > PAGED_GRID) return fail(ctx, G4A_E_SHAPE, "too many rows (%llu)", (unsigned long long)rows);
+    return launch(ctx, kernels[paged_dh(c->Dh)][paged_type(c->kv_type)], dim3(uint32_t(wgs), 2, 1), dim3(256, 1, 1), p, what,
+                  true);
 }
 
 }  // namespace
@@ -2445,8 +2487,9 @@ int g4a_attn_producer_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4
         return fail(ctx, G4A_E_ARG, "rotary_dim %u must be even and <= head_dim %u", rot, cache->Dh);
     if ((a->k == nullptr) != (a->v == nullptr)) return fail(ctx, G4A_E_ARG, "k and v come together");
     if (a->Hq == 0 || a->Hq > 65536) return fail(ctx, G4A_E_UNSUPPORTED, "Hq %u is not 1 .. 65536", a->Hq);
-    p.heads = a->Hq + (a->k ? 2 * cache->Hkv : 0);
-    const uint64_t rows = uint64_t(a->T) * p.heads;
+    const bool quant = a->k && paged_quant(cache->kv_type);
+    p.heads = a->Hq + (a->k && !quant ? 2 * cache->Hkv : 0);
+    const uint64_t rows = uint64_t(a->T) * (a->Hq + (a->k ? 2 * cache->Hkv : 0));
     if (a->T == 0) return G4A_OK;
     if (!a->q || !a->q_out || !a->positions || (a->k && !a->slots))
         return fail(ctx, G4A_E_ARG, "null q / q_out / positions / slots");
@@ -2463,7 +2506,10 @@ int g4a_attn_producer_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4
     p.heads_per_wave = turns * at_once;
     p.groups = (p.heads + p.heads_per_wave - 1) / p.heads_per_wave;
     const uint64_t wgs = (uint64_t(a->T) * p.groups + 3) / 4;
-    if (wgs > PAGED_GRID) return fail(ctx, G4A_E_SHAPE, "too many rows (%llu)", (unsigned long long)rows);
+    // (8 and 4 bits: waves of their own for the K and V rows, behind those of the query rows)
+    const uint32_t kv_groups = quant ? (cache->Hkv + at_once - 1) / at_once : 0;
+    const uint64_t kv_wgs = (uint64_t(a->T) * 2 * kv_groups + 3) / 4;
+    if (wgs + kv_wgs > PAGED_GRID) return fail(ctx, G4A_E_SHAPE, "too many rows (%llu)", (unsigned long long)rows);
     if (rot)
         if (int rc = freq_table(ctx, a->theta, rot, &p.freq)) return rc;
     p.q = a->q;
@@ -2478,8 +2524,15 @@ int g4a_attn_producer_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4
     p.Hq = a->Hq;
     p.rotary_dim = rot;
     p.eps = a->eps;
-    return launch(ctx, ctx->paged_producer[paged_dh(cache->Dh)][cache->kv_type], dim3(uint32_t(wgs), 1, 1),
-                  dim3(256, 1, 1), p, "paged producer", true);
+    hipFunction_t* const kernels = ctx->paged_producer[paged_dh(cache->Dh)];
+    if (quant) {
+        const G4aPagedQuantProducerParams qp{p, uint32_t(wgs), kv_groups};
+        return launch(ctx, kernels[paged_type(cache->kv_type)], dim3(uint32_t(wgs + kv_wgs), 1, 1), dim3(256, 1, 1), qp,
+                      "paged producer", true);
+    }
+    // (query rows alone do not touch the pools)
+    return launch(ctx, kernels[a->k ? paged_type(cache->kv_type) : 0], dim3(uint32_t(wgs), 1, 1), dim3(256, 1, 1), p,
+                  "paged producer", true);
 }
 
 int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_paged_attn_args* a) {
@@ -2511,7 +2564,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.min_part = PAGED_MIN_PART;
     p.scale = a->scale;
     p.softcap = a->attn_softcap;
-    const int d = paged_dh(cache->Dh), t = int(cache->kv_type);
+    const int d = paged_dh(cache->Dh), t = paged_type(cache->kv_type);
     const uint32_t resident = uint32_t(std::max(ctx->cu_count, 1)) * PAGED_WGS_PER_CU[d][t][h];
     // Parts to aim at where there are many units: at 512 dims and up to 8 heads half as many more, which the
     // second workgroup that a CU has room for takes (256 sequences of up to 1500 tokens, f32: 114 us with them,
@@ -2572,6 +2625,16 @@ int g4a_kv_gather_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, uint32_t seq
     if (n == 0) return G4A_OK;
     if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
         return fail(ctx, G4A_E_ARG, "k_out / v_out null or not 16-byte aligned");
+    if (paged_quant(cache->kv_type)) {
+        G4aPagedRowsParams r{};
+        r.c = p.c;
+        r.k_out = k_out;
+        r.v_out = v_out;
+        r.seq = seq;
+        r.pos0 = pos0;
+        r.T = n;
+        return paged_rows(ctx, cache, ctx->paged_read, r, "paged gather");
+    }
     p.k_out = k_out;
     p.v_out = v_out;
     p.seq = seq;
@@ -2582,7 +2645,54 @@ int g4a_kv_gather_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, uint32_t seq
     const uint32_t groups = ((pos0 + n - 1) >> p.rows_shift) - (pos0 >> p.rows_shift) + 1;
     if (groups > PAGED_GRID)
         return fail(ctx, G4A_E_SHAPE, "%u tokens: a gather takes %u groups of %u", n, PAGED_GRID, 1u << p.rows_shift);
-    return launch(ctx, ctx->paged_gather[cache->kv_type], dim3(groups, 2, 1), dim3(256, 1, 1), p, "paged gather", true);
+    return launch(ctx, ctx->paged_gather[paged_type(cache->kv_type)], dim3(groups, 2, 1), dim3(256, 1, 1), p, "paged gather",
+                  true);
+}
+
+int g4a_kv_page_bytes(g4a_ctx* ctx, const g4a_paged_cache* cache, uint64_t* bytes) {
+    QueryScope q(ctx);
+    if (!bytes) return fail(ctx, G4A_E_ARG, "null bytes");
+    if (!cache) return fail(ctx, G4A_E_ARG, "null cache");
+    // (a question about the widths, asked before there are pools)
+    g4a_paged_cache c = *cache;
+    alignas(16) static char somewhere[16];
+    c.k_pages = c.v_pages = somewhere;
+    c.n_pages = 1;
+    c.ring = 0;
+    G4aPaged p;
+    if (int rc = paged_cache(ctx, &c, false, true, &p)) return rc;
+    *bytes = p.page_stride * (c.kv_type == G4A_KV_F32 ? 4 : c.kv_type == G4A_KV_BF16 ? 2 : 1);
+    return G4A_OK;
+}
+
+int g4a_kv_write_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const float* k, const float* v, const uint32_t* slots,
+                       uint32_t T) {
+    if (!ctx) return fail(ctx, G4A_E_ARG, "null ctx");
+    G4aPagedRowsParams p{};
+    if (int rc = paged_cache(ctx, cache, false, true, &p.c)) return rc;
+    if (T == 0) return G4A_OK;
+    if (!k || !v || !slots || !aligned16(k) || !aligned16(v) || !aligned4({slots}))
+        return fail(ctx, G4A_E_ARG, "k / v null or not 16-byte aligned, or slots null or not 4-byte aligned");
+    p.k_in = k;
+    p.v_in = v;
+    p.slots = slots;
+    p.T = T;
+    return paged_rows(ctx, cache, ctx->paged_write, p, "paged write");
+}
+
+int g4a_kv_read_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const uint32_t* slots, uint32_t T, float* k_out,
+                      float* v_out) {
+    if (!ctx) return fail(ctx, G4A_E_ARG, "null ctx");
+    G4aPagedRowsParams p{};
+    if (int rc = paged_cache(ctx, cache, false, true, &p.c)) return rc;
+    if (T == 0) return G4A_OK;
+    if (!k_out || !v_out || !slots || !aligned16(k_out) || !aligned16(v_out) || !aligned4({slots}))
+        return fail(ctx, G4A_E_ARG, "k_out / v_out null or not 16-byte aligned, or slots null or not 4-byte aligned");
+    p.k_out = k_out;
+    p.v_out = v_out;
+    p.slots = slots;
+    p.T = T;
+    return paged_rows(ctx, cache, ctx->paged_read, p, "paged read");
 }
 
 struct g4a_graph {

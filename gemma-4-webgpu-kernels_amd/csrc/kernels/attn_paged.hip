@@ -52,6 +52,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 template <int DH, typename KV, int NHQ>
 struct PagedCfg {
     static constexpr bool BF = sizeof(KV) == 2;
+    static constexpr int DIMS = DH;
     static constexpr int HR = 4 * NHQ;                       // query heads of a unit
     static constexpr int EL = 16 / (int)sizeof(KV);          // values of a 16-byte load
     static constexpr int KC = DH / (4 * EL);                 // K loads of a tile
@@ -137,6 +138,77 @@ __device__ __forceinline__ uint32_t load_scalar(const uint32_t* p, size_t i) {
 __device__ __forceinline__ size_t uniform(size_t x) {
     return (size_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
            (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
+// This workgroup's part: tiles from .. to - 1 of sequence b's, one of `parts` of its unit of the query heads h0 .. h0 +
+// nh - 1 over kv head kvh. False where it has none. `lens`: LDS for PAGED_SEQS words.
+struct PagedPart {
+    PagedSpan sp;
+    uint32_t b, parts, from, to, kvh, h0, nh;
+};
+
+template <int HR>
+__device__ __forceinline__ bool paged_find(const G4aPagedAttnParams& p, uint32_t* lens, int lane, int w, PagedPart& x) {
+    // every wave sums the lengths, a span of `each` sequences a lane
+    const uint32_t n = p.c.n_seqs, each = (n + 63) / 64;
+    const uint32_t my_len = lane < (int)n && each == 1 ? p.c.len[lane] : 0u;
+    // (more than one a lane: through LDS, by every wave alike. Short loops: sixteen lengths a lane in registers,
+    // unrolled, took 1.6 us more of a small call, in code that no cache holds yet.)
+    if (each > 1)
+        for (uint32_t b = lane; b < n; b += 64) lens[b] = p.c.len[b];
+    auto lane_tiles = [&](uint32_t b) { return b < n ? paged_span(p, each == 1 ? my_len : lens[b]).n : 0u; };
+    uint32_t mine = 0;
+    for (uint32_t i = 0; i < each; ++i) mine += lane_tiles(lane * each + i);
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane(wave_incl_sum(mine), 63) * p.units;
+    // (not in whole rounds of the waves: 64 windows of 512, hd 256 f32, took 23.4 us so, 21.1 with parts of five tiles)
+    uint32_t quota = max((total + p.spread - 1) / p.spread, p.min_part), upto;
+    // parts of a sequence's units; the first few quotas may give more parts than `fit` holds, the last cannot
+    auto lane_parts = [&](uint32_t b) { return b < n ? p.units * paged_parts(lane_tiles(b), quota) : 0u; };
+    for (int tries = 0;; ++tries) {
+        mine = 0;
+        for (uint32_t i = 0; i < each; ++i) mine += lane_parts(lane * each + i);
+        upto = wave_incl_sum(mine);
+        if (p.fit == 0 || (uint32_t)__builtin_amdgcn_readlane(upto, 63) <= p.fit) break;
+        const uint32_t sure = (total + p.fit - n * p.units - 1) / (p.fit - n * p.units);
+        quota = tries < 3 ? min(quota + (quota + 31) / 32, sure) : sure;
+    }
+    if (blockIdx.x == 0 && w == 0) {  // where each sequence's parts start, for the merge
+        if (lane == 0) p.offs[0] = quota;
+        uint32_t before = upto - mine;
+        for (uint32_t i = 0; i < each; ++i) {
+            const uint32_t b = lane * each + i;
+            if (b < n) p.offs[1 + b] = before;
+            before += lane_parts(b);
+        }
+    }
+    const uint32_t at = blockIdx.x;
+    if (at >= (uint32_t)__builtin_amdgcn_readlane(upto, 63)) return false;
+    // the sequence it is of, and that one's first part
+    const int l0 = __builtin_ctzll(__ballot(upto > at));
+    x.b = l0 * each;
+    uint32_t base = __builtin_amdgcn_readlane(upto - mine, l0), len;
+    if (each == 1) {
+        len = __builtin_amdgcn_readlane(my_len, x.b);
+    } else {
+        static_assert(PAGED_SEQS <= 64 * 64, "a lane's span of sequences, a lane each");
+        const uint32_t mine_of = lane < (int)min(each, n - x.b) ? lane_parts(x.b + lane) : 0u;
+        const uint32_t incl = wave_incl_sum(mine_of);
+        const int l1 = __builtin_ctzll(__ballot(base + incl > at));
+        base += __builtin_amdgcn_readlane(incl - mine_of, l1);
+        x.b += l1;
+        len = __builtin_amdgcn_readfirstlane(lens[x.b]);
+        barrier_lds();  // every wave has read the lengths: what comes next goes there
+    }
+    x.sp = paged_span(p, len);
+    x.parts = __builtin_amdgcn_readfirstlane(paged_parts(x.sp.n, quota));
+    const uint32_t j = (at - base) / x.parts, part = at - base - j * x.parts;
+    const uint32_t floor = x.sp.n / x.parts, more = x.sp.n % x.parts;
+    x.from = part * floor + min(part, more);
+    x.to = x.from + floor + (part < more ? 1u : 0u);
+    x.kvh = j / p.chunks;
+    x.h0 = x.kvh * p.group + (j - x.kvh * p.chunks) * HR;
+    x.nh = min((uint32_t)HR, p.group - (j - x.kvh * p.chunks) * HR);
+    return true;
 }
 
 // A tile of K or V: `bytes` from its first row on, behind which nothing is read. Buffer loads:
@@ -352,63 +424,12 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
     const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, key = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    // ---- this workgroup's part: every wave sums the lengths, a span of `each` sequences a lane ----
-    const uint32_t n = c.n_seqs, each = (n + 63) / 64;
-    const uint32_t my_len = lane < (int)n && each == 1 ? c.len[lane] : 0u;
-    // (more than one a lane: through LDS, by every wave alike. Short loops: sixteen lengths a lane in registers,
-    // unrolled, took 1.6 us more of a small call, in code that no cache holds yet.)
-    uint32_t* const lens = reinterpret_cast<uint32_t*>(smem);
-    if (each > 1)
-        for (uint32_t b = lane; b < n; b += 64) lens[b] = c.len[b];
-    auto lane_tiles = [&](uint32_t b) { return b < n ? paged_span(p, each == 1 ? my_len : lens[b]).n : 0u; };
-    uint32_t mine = 0;
-    for (uint32_t i = 0; i < each; ++i) mine += lane_tiles(lane * each + i);
-    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane(wave_incl_sum(mine), 63) * p.units;
-    // (not in whole rounds of the waves: 64 windows of 512, hd 256 f32, took 23.4 us so, 21.1 with parts of five tiles)
-    uint32_t quota = max((total + p.spread - 1) / p.spread, p.min_part), upto;
-    // parts of a sequence's units; the first few quotas may give more parts than `fit` holds, the last cannot
-    auto lane_parts = [&](uint32_t b) { return b < n ? p.units * paged_parts(lane_tiles(b), quota) : 0u; };
-    for (int tries = 0;; ++tries) {
-        mine = 0;
-        for (uint32_t i = 0; i < each; ++i) mine += lane_parts(lane * each + i);
-        upto = wave_incl_sum(mine);
-        if (p.fit == 0 || (uint32_t)__builtin_amdgcn_readlane(upto, 63) <= p.fit) break;
-        const uint32_t sure = (total + p.fit - n * p.units - 1) / (p.fit - n * p.units);
-        quota = tries < 3 ? min(quota + (quota + 31) / 32, sure) : sure;
-    }
-    if (blockIdx.x == 0 && w == 0) {  // where each sequence's parts start, for the merge
-        if (lane == 0) p.offs[0] = quota;
-        uint32_t before = upto - mine;
-        for (uint32_t i = 0; i < each; ++i) {
-            const uint32_t b = lane * each + i;
-            if (b < n) p.offs[1 + b] = before;
-            before += lane_parts(b);
-        }
-    }
-    const uint32_t at = blockIdx.x;
-    if (at >= (uint32_t)__builtin_amdgcn_readlane(upto, 63)) return;
-    // the sequence it is of, and that one's first part
-    const int l0 = __builtin_ctzll(__ballot(upto > at));
-    uint32_t b = l0 * each, base = __builtin_amdgcn_readlane(upto - mine, l0), len;
-    if (each == 1) {
-        len = __builtin_amdgcn_readlane(my_len, b);
-    } else {
-        static_assert(PAGED_SEQS <= 64 * 64, "a lane's span of sequences, a lane each");
-        const uint32_t mine_of = lane < (int)min(each, n - b) ? lane_parts(b + lane) : 0u;
-        const uint32_t incl = wave_incl_sum(mine_of);
-        const int l1 = __builtin_ctzll(__ballot(base + incl > at));
-        base += __builtin_amdgcn_readlane(incl - mine_of, l1);
-        b += l1;
-        len = __builtin_amdgcn_readfirstlane(lens[b]);
-        barrier_lds();  // every wave has read the lengths: the query rows go there
-    }
-    const PagedSpan sp = paged_span(p, len);
-    const uint32_t parts = __builtin_amdgcn_readfirstlane(paged_parts(sp.n, quota));
-    const uint32_t j = (at - base) / parts, part = at - base - j * parts;
-    const uint32_t floor = sp.n / parts, more = sp.n % parts;
-    const uint32_t s = part * floor + min(part, more), e = s + floor + (part < more ? 1u : 0u);  // its tiles
-    const uint32_t kvh = j / p.chunks, h0 = kvh * p.group + (j - kvh * p.chunks) * HR;
-    const uint32_t nh = min((uint32_t)HR, p.group - (j - kvh * p.chunks) * HR);
+    // ---- this workgroup's part ----
+    PagedPart mine;
+    if (!paged_find<HR>(p, reinterpret_cast<uint32_t*>(smem), lane, w, mine)) return;
+    const PagedSpan sp = mine.sp;
+    const uint32_t at = blockIdx.x, b = mine.b, parts = mine.parts, s = mine.from, e = mine.to, kvh = mine.kvh, h0 = mine.h0,
+                   nh = mine.nh;
     if (sp.n == 0) {
         for (uint32_t i = tid; i < nh * DH; i += 256) p.out[((size_t)b * p.Hq + h0) * DH + i] = 0.0f;
         return;
@@ -776,9 +797,9 @@ __device__ __forceinline__ void paged_decode(const G4aPagedAttnParams& p) {
 // in LDS.
 constexpr int PAGED_PARTS = 1024;  // of a unit, at most
 
-template <int DH, typename KV, int NHQ, int CI, int W>
+template <typename C, int CI, int W>
 __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
-    using C = PagedCfg<DH, KV, NHQ>;
+    constexpr int DH = C::DIMS, NHQ = C::HR / 4;
     constexpr int NT = 64 * W, CG = NT / CI;
     static_assert(CI == 16 || CI == 64, "a wave's groups meet by columns of 16 lanes");
     __shared__ f4v w_s[PAGED_PARTS];
@@ -864,9 +885,9 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
     extern "C" __global__ __launch_bounds__(256, occ) void g4a_paged_decode_win_d##dh##_##type##_h##nhq(      \
         G4aPagedAttnParams p) { paged_decode<dh, kv, nhq, true>(p); }                                         \
     extern "C" __global__ __launch_bounds__(512) void g4a_paged_combine16_d##dh##_##type##_h##nhq(            \
-        G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 16, 8>(p); }                                      \
+        G4aPagedAttnParams p) { paged_combine<PagedCfg<dh, kv, nhq>, 16, 8>(p); }                                      \
     extern "C" __global__ __launch_bounds__(256) void g4a_paged_combine64_d##dh##_##type##_h##nhq(            \
-        G4aPagedAttnParams p) { paged_combine<dh, kv, nhq, 64, 4>(p); }
+        G4aPagedAttnParams p) { paged_combine<PagedCfg<dh, kv, nhq>, 64, 4>(p); }
 #define G4A_PAGED_DECODE_TYPES(dh, nhq, occ_f32, occ_bf16) \
     G4A_PAGED_DECODE(dh, f32, float, nhq, occ_f32)         \
     G4A_PAGED_DECODE(dh, bf16, __bf16, nhq, occ_bf16)

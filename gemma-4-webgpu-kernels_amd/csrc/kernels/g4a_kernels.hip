@@ -9,3 +9,5 @@
 #include "elementwise.hip"
 #include "paged.hip"
 #include "attn_paged.hip"
+#include "paged_rows.hip"
+#include "attn_paged_quant.hip"

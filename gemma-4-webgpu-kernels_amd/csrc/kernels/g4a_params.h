@@ -346,7 +346,7 @@ struct G4aEmbedF32Params {
 // ring: modulo per_seq), at row t & (page size - 1) of it; a row is Hkv * Dh values.
 // An entry of n_pages or more names no page.
 struct G4aPaged {
-    void* k;                // [n_pages] pages, page_stride values apart, f32 or bf16
+    void* k;                // [n_pages] pages, page_stride values (8 and 4 bits: bytes) apart
     void* v;
     uint32_t* table;        // device [n_seqs][per_seq]
     const uint32_t* len;    // device [n_seqs]: tokens in the cache
@@ -393,7 +393,28 @@ struct G4aPagedProducerParams {
     float eps;
 };
 
-// Tokens [pos0, pos0 + n) of sequence seq in order, as f32 (g4a_paged_gather_*).
+// Rows of K and V between f32 arrays and the pages: by slot (g4a_paged_write_*, g4a_paged_read_*), or a sequence's
+// tokens in order (g4a_paged_gather_d*).
+struct G4aPagedRowsParams {
+    G4aPaged c;
+    const float* k_in;       // [T, Hkv, Dh]
+    const float* v_in;
+    float* k_out;
+    float* v_out;
+    const uint32_t* slots;   // device [T], or null: tokens pos0 .. of sequence seq
+    uint32_t seq, pos0;
+    uint32_t T;
+    uint32_t turns;          // of a wave, one after the other
+};
+
+// The producer into pages of 8 and 4 bits (g4a_paged_producer_d*_{i8,i4}): workgroups below q_wgs take the query rows,
+// as p.heads = p.Hq says, those behind them the K and V rows, of which a token has 2 kv_groups waves' work.
+struct G4aPagedQuantProducerParams {
+    G4aPagedProducerParams p;
+    uint32_t q_wgs, kv_groups;
+};
+
+// Tokens [pos0, pos0 + n) of sequence seq in order, as f32 (g4a_paged_gather_{f32,bf16}).
 struct G4aPagedGatherParams {
     G4aPaged c;
     float* k_out;            // [n, Hkv, Dh]

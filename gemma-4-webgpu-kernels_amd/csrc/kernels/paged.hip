@@ -8,6 +8,7 @@
 
 #include "g4a_math.h"
 #include "g4a_params.h"
+#include "paged_quant.h"
 
 namespace {
 
@@ -211,7 +212,6 @@ __device__ __forceinline__ void page_map(const G4aPageMapParams& p) {
 }
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Four values of a page's row, rounded to nearest even where the page holds bf16.
 __device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }

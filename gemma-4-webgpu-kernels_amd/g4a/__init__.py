@@ -25,7 +25,7 @@ G4A_OK = 0
 # G4A_NOALLOC_SCRATCH_BYTES of include/g4a.h: the static scratch of g4a_attention_noalloc
 NOALLOC_SCRATCH_BYTES = 64 << 20
 # g4a_kv_type, G4A_NO_ROW and G4A_SEQ_END of include/g4a.h
-KV_TYPES = {"f32": 0, "bf16": 1}
+KV_TYPES = {"f32": 0, "bf16": 1, "i4": 4, "i8": 8}
 NO_ROW = SEQ_END = 0xFFFFFFFF
 KERNEL_NAMES = {0: "none", 1: "decode", 2: "prefill", 3: "generic", 4: "decode_short"}
 
@@ -185,6 +185,9 @@ def load_library(path: Path = LIB_PATH) -> ctypes.CDLL:
         "g4a_attn_producer_paged": (c_int, [ctxp, ctypes.POINTER(PagedCache), ctypes.POINTER(PagedProducerArgs)]),
         "g4a_attention_paged": (c_int, [ctxp, ctypes.POINTER(PagedCache), ctypes.POINTER(PagedAttnArgs)]),
         "g4a_kv_gather_paged": (c_int, [ctxp, ctypes.POINTER(PagedCache)] + [ctypes.c_uint32] * 3 + [vp, vp]),
+        "g4a_kv_page_bytes": (c_int, [ctxp, ctypes.POINTER(PagedCache), ctypes.POINTER(ctypes.c_uint64)]),
+        "g4a_kv_write_paged": (c_int, [ctxp, ctypes.POINTER(PagedCache), vp, vp, vp, ctypes.c_uint32]),
+        "g4a_kv_read_paged": (c_int, [ctxp, ctypes.POINTER(PagedCache), vp, ctypes.c_uint32, vp, vp]),
         "g4a_timer_start": (c_int, [ctxp]),
         "g4a_timer_stop": (c_int, [ctxp, ctypes.POINTER(ctypes.c_float)]),
         "g4a_get_device_info": (c_int, [ctxp, ctypes.POINTER(DeviceInfo)]),
@@ -510,6 +513,20 @@ class Context:
     def kv_gather_paged(self, cache: PagedCache, seq: int, pos0: int, n: int, k_out: int, v_out: int) -> None:
         """g4a_kv_gather_paged: tokens pos0 .. pos0 + n - 1 of a sequence in order, as f32 rows."""
         self._check(self.lib.g4a_kv_gather_paged(self.handle, cache, seq, pos0, n, k_out, v_out))
+
+    def kv_write_paged(self, cache: PagedCache, k: int, v: int, slots: int, T: int) -> None:
+        """g4a_kv_write_paged: f32 rows of T tokens into their slots, in the pages' type."""
+        self._check(self.lib.g4a_kv_write_paged(self.handle, cache, k, v, slots, T))
+
+    def kv_read_paged(self, cache: PagedCache, slots: int, T: int, k_out: int, v_out: int) -> None:
+        """g4a_kv_read_paged: the rows at T slots as f32."""
+        self._check(self.lib.g4a_kv_read_paged(self.handle, cache, slots, T, k_out, v_out))
+
+    def kv_page_bytes(self, cache: PagedCache) -> int:
+        """g4a_kv_page_bytes: bytes from one page of a pool to the next (host only)."""
+        n = ctypes.c_uint64()
+        self._check(self.lib.g4a_kv_page_bytes(self.handle, cache, ctypes.byref(n)))
+        return n.value
 
     # ---- graph capture (launch-bound sequences) ----
     def capture_begin(self) -> None:

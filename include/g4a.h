@@ -407,7 +407,7 @@ int g4a_embed_rows_q(g4a_ctx *ctx, const g4a_qweight *table, const uint32_t *ids
  * it on the context's stream with the same pointers and arguments.
  * Capturable: attention with contiguous positions (q_pos0 / k_pos0), the
  * producer and norm/RoPE calls with contiguous positions, kv_write, every
- * projection, elementwise and norm op, and the paged cache's four calls. A call
+ * projection, elementwise and norm op, and the paged cache's calls. A call
  * that needs host staging
  * (explicit position arrays, embedding ids), a larger workspace or a new RoPE
  * table, and g4a_h2d / g4a_d2h / g4a_zero / g4a_sync / the timers, fail with
@@ -483,8 +483,8 @@ int g4a_u32_add(g4a_ctx *ctx, uint32_t *counters, uint32_t n, uint32_t inc);
  * block_table[b * pages_per_seq + t / page_size]; with `ring` the table is a ring
  * (entry t / page_size % pages_per_seq) that holds a sequence's last
  * pages_per_seq * page_size tokens, as a sliding layer needs. A page is page_size
- * rows of [Hkv, Dh] values, K and V in pools of their own; an entry of n_pages or
- * more names no page, and tokens on it are treated as absent. Layers that share
+ * rows of [Hkv, Dh] values (8 and 4 bits: see g4a_kv_type), K and V in pools of their own;
+ * an entry of n_pages or more names no page, and tokens on it are treated as absent. Layers that share
  * tables and lengths differ in their pools alone. Pages may be shared between
  * sequences (a common prefix) as long as nobody writes into them.
  *
@@ -496,9 +496,28 @@ int g4a_u32_add(g4a_ctx *ctx, uint32_t *counters, uint32_t n, uint32_t inc);
 #define G4A_NO_ROW 0xFFFFFFFFu  /* no slot, no position */
 #define G4A_SEQ_END 0xFFFFFFFFu /* in new_len: the sequence ends */
 
+/* What the pages hold. Every operator computes in f32 or more on the values that a page
+ * stands for. 8 and 4 bits: each row (one token's K or V of one head) holds whole numbers n
+ * and scales, made as it is written:
+ *   8 bits: value = S n, -127 <= n <= 127, S the least bfloat16 with 127 S >= max |x| of the row;
+ *   4 bits: value = S sub n, in groups of 32 dims with a whole number sub of their own:
+ *     -8 <= n <= 7, S the least bfloat16 with 1016 S >= max |x| of the row, |sub| the least whole
+ *     number >= 1 with 8 |sub| S >= max |x| of the group, sub's sign such that the group's extreme
+ *     (the positive of two equal ones) stands at n = -8.
+ * S is at least 2^-126; n is the exact quotient rounded to nearest, halves to even, and cut to
+ * its range. So a value is off by at most half a step (S, or S |sub|); in 4 bits, at the end
+ * opposite to its group's extreme, by at most one. A row that holds an infinity or a NaN reads as
+ * NaN throughout; magnitudes within 2^-7 of f32's largest may read as infinity.
+ *
+ * Layout of such a page, in bytes: rows [Hkv][page_size] of Dh * bits / 8, n + 2^(bits - 1) stored, in
+ * 4 bits an even dim in the low half of its byte; then [Hkv][page_size / 16] blocks: in 4 bits
+ * sub + 128 of 16 tokens' G = Dh / 32 groups (K: [token][place], group g at place g % 4 * (G / 4) + g / 4, at
+ * Dh 64 at g; V: [group][token]), then S of 16 tokens. The whole is rounded up to 128 bytes. */
 typedef enum g4a_kv_type {
     G4A_KV_F32 = 0,
-    G4A_KV_BF16 = 1, /* rounded to nearest even on writing; every operator computes in f32 */
+    G4A_KV_BF16 = 1, /* rounded to nearest even on writing */
+    G4A_KV_I4 = 4,
+    G4A_KV_I8 = 8,
 } g4a_kv_type;
 
 typedef struct g4a_paged_cache {
@@ -506,7 +525,8 @@ typedef struct g4a_paged_cache {
     void *v_pages;
     uint32_t *block_table; /* device [n_seqs, pages_per_seq] */
     uint32_t *kv_len;      /* device [n_seqs]: tokens of each sequence */
-    uint64_t page_stride;  /* values from one page to the next, a multiple of 8; 0: page_size * Hkv * Dh */
+    uint64_t page_stride;  /* values from one page to the next, a multiple of 8; 0: page_size * Hkv * Dh.
+                              8 and 4 bits: bytes, a multiple of 16; 0: g4a_kv_page_bytes */
     uint32_t n_seqs, pages_per_seq;
     uint32_t n_pages;      /* n_pages * page_size < 2^32 */
     uint32_t page_size;    /* tokens, a power of two from 16 to 65536 */
@@ -515,6 +535,10 @@ typedef struct g4a_paged_cache {
     uint32_t kv_type;      /* g4a_kv_type */
     uint32_t ring;         /* 0, or 1: the tables are rings */
 } g4a_paged_cache;
+
+/* Bytes from one page of a pool to the next, from page_size, Hkv, Dh, kv_type and page_stride (a query: no GPU work,
+ * ctx may be NULL, the pointers and counts are not looked at): a pool is n_pages times as many. */
+int g4a_kv_page_bytes(g4a_ctx *ctx, const g4a_paged_cache *cache, uint64_t *bytes);
 
 /* The pages, slots and positions of one step, from lengths on the device.
  * Sequence b (kv_len[b] tokens so far) adds new_len[b] tokens: pages it lacks are
@@ -569,7 +593,9 @@ int g4a_page_map(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4a_page_map_
  * included; slot G4A_NO_ROW (or one past the pool) writes no K and V. The slots
  * of a call differ from each other. k = v = NULL: only q. Of the cache the pools
  * and widths are used. A (theta, rotary_dim) pair's first use must be outside a
- * capture. */
+ * capture. Into pages of 8 and 4 bits K and V rows go in 64 bits up to one rounding to
+ * f32, ahead of the rounding to the page's numbers, so that these do not depend on an order
+ * of sums: the same rows give the same pages, also in another batch. */
 typedef struct g4a_paged_producer_args {
     const float *q;      /* [T, Hq, Dh], 16-byte aligned like all rows here */
     const float *k;      /* [T, Hkv, Dh], or NULL */
@@ -595,7 +621,10 @@ int g4a_attn_producer_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4
  * and grid depends on the arguments alone, so a captured call follows lengths and
  * tables. The partial results of sequences that
  * several workgroups share stand in the context's workspace: run the call once, at
- * its sizes, before capturing it. Results are the same bits from call to call. */
+ * its sizes, before capturing it. Results are the same bits from call to call.
+ * On pages of 8 and 4 bits queries and probabilities are held to 2^-22 of their value (or
+ * 2^-35 of the largest of their head's, or of the tokens seen so far), sums in f32; a query row that
+ * holds an infinity or a NaN gives a row of NaN where it sees a token. */
 typedef struct g4a_paged_attn_args {
     const float *q; /* [n_seqs, Hq, Dh], 16-byte aligned */
     float *out;     /* [n_seqs, Hq * Dh], 16-byte aligned */
@@ -611,6 +640,15 @@ int g4a_attention_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4a_pa
  * cache does not hold (past kv_len[seq], lost by a ring, on no page) are zeros. */
 int g4a_kv_gather_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, uint32_t seq, uint32_t pos0, uint32_t n,
                         float *k_out, float *v_out);
+
+/* T tokens' rows k, v [T, Hkv, Dh] (f32, 16-byte aligned) into their slots, in the pages' type and as they are: a
+ * prefix from elsewhere, or from a cache of another type. Rows of slot G4A_NO_ROW (or one past the pool) are left out;
+ * the others differ from each other. Of the cache the pools and widths are used, here and in g4a_kv_read_paged. */
+int g4a_kv_write_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const float *k, const float *v, const uint32_t *slots,
+                       uint32_t T);
+/* The rows at T slots as f32 [T, Hkv, Dh]; zeros for slot G4A_NO_ROW (or one past the pool). */
+int g4a_kv_read_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const uint32_t *slots, uint32_t T, float *k_out,
+                      float *v_out);
 
 /* ---- timing (HIP events on the context's stream) ----------------------- */
 int g4a_timer_start(g4a_ctx *ctx);
