@@ -933,8 +933,7 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
             }
             for (int h = 0; h < 3; ++h) {
                 for (int win = 0; win < 2; ++win) {
-                    snprintf(name, sizeof name, "g4a_paged_decode%s_d%d_%s_h%d", win && t < 2 ? "_win" : "", 64 << d, types[t],
-                             1 << h);
+                    snprintf(name, sizeof name, "g4a_paged_decode%s_d%d_%s_h%d", win ? "_win" : "", 64 << d, types[t], 1 << h);
                     if (int rc = get_fn(ctx, &ctx->paged_decode[win][d][t][h], name)) return bail(rc);
                 }
                 for (int w = 0; w < 2; ++w) {

@@ -53,6 +53,7 @@ template <int DH, typename KV, int NHQ>
 struct PagedCfg {
     static constexpr bool BF = sizeof(KV) == 2;
     static constexpr int DIMS = DH;
+    static __device__ __forceinline__ float exp(float x) { return expf(x); }  // of the partials' maxima
     static constexpr int HR = 4 * NHQ;                       // query heads of a unit
     static constexpr int EL = 16 / (int)sizeof(KV);          // values of a 16-byte load
     static constexpr int KC = DH / (4 * EL);                 // K loads of a tile
@@ -847,7 +848,7 @@ __device__ __forceinline__ void paged_combine(const G4aPagedAttnParams& p) {
             const f4v m = i < NT ? m0 : ml[(size_t)i * 2 * NHQ], l = i < NT ? l0 : ml[(size_t)i * 2 * NHQ + NHQ];
             f4v f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) f[r] = m[r] == G4A_NEG_INF ? 0.0f : expf(m[r] - M[r]);
+            for (int r = 0; r < 4; ++r) f[r] = m[r] == G4A_NEG_INF ? 0.0f : C::exp(m[r] - M[r]);
             w_s[i] = f;
             L += l * f;
         }
