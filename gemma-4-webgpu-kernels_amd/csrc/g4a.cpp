@@ -2560,7 +2560,9 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     if (std::max<uint64_t>(p.span / 16 + 2, item / 64) * cache->n_seqs * p.units >> 31)
         return fail(ctx, G4A_E_SHAPE, "%u sequences of up to %u tokens in %u head groups: at most 2^31 tiles of 16 tokens",
                     cache->n_seqs, p.span, p.units);
-    p.min_part = PAGED_MIN_PART;
+    // (8 and 4 bits of 512 dims and up to 8 heads: eight waves, attn_paged_quant.hip)
+    const uint32_t waves = paged_quant(cache->kv_type) && cache->Dh == 512 && h < 2 ? 8 : 4;
+    p.min_part = std::max(PAGED_MIN_PART, waves);
     p.scale = a->scale;
     p.softcap = a->attn_softcap;
     const int d = paged_dh(cache->Dh), t = paged_type(cache->kv_type);
@@ -2579,7 +2581,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     // workgroups a CU, 41.4 with three, 49.9 with two.)
     auto shares = [&](uint32_t seqs, uint32_t* spread, uint32_t* fit) {
         const uint64_t units = uint64_t(seqs) * p.units, tiles = uint64_t(p.span / 16 + 2) * units;
-        const uint64_t most_parts = std::min<uint64_t>(std::min(resident, PAGED_MAX_PARTS), tiles / PAGED_MIN_PART + units);
+        const uint64_t most_parts = std::min<uint64_t>(std::min(resident, PAGED_MAX_PARTS), tiles / p.min_part + units);
         *fit = (PAGED_WGS_PER_CU[d][t][h] >= 3 ? 3 : 2) * units <= most_parts ? uint32_t(most_parts) : 0;
         *spread = uint32_t(std::max<uint64_t>(1, *fit ? most_parts : std::min<uint64_t>(over, PAGED_MAX_PARTS - 1)));
         return *fit ? *fit : uint32_t(*spread + units);  // the workgroups
@@ -2593,7 +2595,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.part_ml = p.part + size_t(slots) * item;
     // whether a unit can have more tiles than the smallest part (a window's tokens may start inside a tile, and so
     // may a ring's)
-    const bool splits = (p.span < p.room || cache->ring ? (p.span + 14) / 16 + 1 : (p.room + 15) / 16) > PAGED_MIN_PART;
+    const bool splits = (p.span < p.room || cache->ring ? (p.span + 14) / 16 + 1 : (p.room + 15) / 16) > p.min_part;
     const G4aPagedAttnParams all = p;
     for (uint32_t b0 = 0; b0 < cache->n_seqs; b0 += most) {
         p.c.n_seqs = std::min(most, cache->n_seqs - b0);
@@ -2602,7 +2604,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
         p.q = all.q + size_t(b0) * a->Hq * cache->Dh;
         p.out = all.out + size_t(b0) * a->Hq * cache->Dh;
         const uint32_t wgs = shares(p.c.n_seqs, &p.spread, &p.fit), units = p.c.n_seqs * p.units;
-        if (int rc = launch(ctx, ctx->paged_decode[a->sliding_window != 0][d][t][h], dim3(wgs, 1, 1), dim3(256, 1, 1), p,
+        if (int rc = launch(ctx, ctx->paged_decode[a->sliding_window != 0][d][t][h], dim3(wgs, 1, 1), dim3(64 * waves, 1, 1), p,
                             "paged decode", true))
             return rc;
         if (!splits) continue;

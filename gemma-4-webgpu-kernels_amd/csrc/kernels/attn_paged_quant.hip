@@ -5,8 +5,6 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <type_traits>
-
 #include "g4a_math.h"
 #include "g4a_params.h"
 #include "paged_quant.h"
@@ -21,9 +19,10 @@ struct QuantCfg {
     static constexpr int EV = DH / 16 < 32 / (BITS / 4) ? DH / 16 : 32 / (BITS / 4);  // dims of a lane and block
     static constexpr int NA = DH / 16;                                // accumulators of a lane, of 16 rows
     static constexpr int ITEMS = NHQ * DH;                            // (4 heads, dim) of a partial
-    static constexpr int ML = 16 * NHQ;                               // lanes that hand accumulators over
+    static constexpr int ML = 16 * NHQ;                               // lanes with a row of heads each, per accumulator
+    static constexpr int W = DH == 512 && NHQ < 4 ? 8 : 4;            // waves
     // the queries (two fp16 parts), the waves' accumulators and the sequences' lengths never live at once
-    static constexpr int SM0 = 4 * HR * DH > 4 * NA * ML * 16 ? 4 * HR * DH : 4 * NA * ML * 16;
+    static constexpr int SM0 = 4 * HR * DH > W * NA * ML * 16 ? 4 * HR * DH : W * NA * ML * 16;
     static constexpr int SM = SM0 > 4096 ? SM0 : 4096;
     static_assert(SM >= 4 * (int)PAGED_SEQS, "the lengths of PAGED_SEQS sequences");
     // Items in the accumulators' order: 4 heads hq, accumulator a, lane n of 16.
@@ -92,19 +91,19 @@ __device__ __forceinline__ uint32_t byte_fields(uint32_t w) {
 constexpr float LOG2E = 0x1.715476p+0f;
 // Scores are relative to a maximum that follows the tiles' by more than this (of 2^x) alone: the accumulators are
 // scaled then, which took a fifth of a tile's vector instructions where every new maximum did.
-constexpr float LAZY = 4.0f;
+constexpr float LAZY = 8.0f;
 
 template <int DH, int BITS, int NHQ, bool WIN>
 __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) {
     using C = QuantCfg<DH, BITS, NHQ>;
     using Q = QuantRow<DH, BITS>;
     constexpr bool I4 = BITS == 4;
-    constexpr int HR = C::HR, NA = C::NA, EV = C::EV, ROW = Q::ROW, G = Q::G, ML = C::ML, COLS = 2 * HR;
+    constexpr int HR = C::HR, NA = C::NA, EV = C::EV, ROW = Q::ROW, G = Q::G, ML = C::ML, COLS = 2 * HR, W = C::W;
     constexpr int KL = ROW >= 64 ? ROW / 64 : 1, KW = ROW >= 64 ? 4 : 2;      // K: loads of a lane, words of one
     constexpr int VN = DH / (16 * EV), VBY = EV * BITS / 8, VW = VBY / 4;     // V: blocks of dims, a lane's bytes and words
     __shared__ __attribute__((aligned(16))) char smem[C::SM];
-    __shared__ __attribute__((aligned(16))) float f_s[4][HR];
-    __shared__ float m_s[4][HR], l_s[4][HR], r_s[4], k_s[HR];
+    __shared__ __attribute__((aligned(16))) float f_s[W][HR];
+    __shared__ float m_s[W][HR], l_s[W][HR], r_s[W], k_s[HR];
     f16x8* const qs = reinterpret_cast<f16x8*>(smem);
     f4v* const mrg = reinterpret_cast<f4v*>(smem);
     const G4aPaged& c = p.c;
@@ -115,7 +114,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     const PagedSpan sp = mine.sp;
     const uint32_t at = blockIdx.x, b = mine.b, e = mine.to, h0 = mine.h0, nh = mine.nh, kvh = mine.kvh;
     if (sp.n == 0) {
-        for (uint32_t i = tid; i < nh * DH; i += 256) p.out[((size_t)b * p.Hq + h0) * DH + i] = 0.0f;
+        for (uint32_t i = tid; i < nh * DH; i += 64 * W) p.out[((size_t)b * p.Hq + h0) * DH + i] = 0.0f;
         return;
     }
 
@@ -127,9 +126,12 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     struct Tile {
         PagedTile rows, meta;
     };
-    auto tile_of = [&](const void* pool, uint32_t page, uint32_t t) {
+    // (`is` false: of no bytes, whose loads go nowhere. One copy of a tile's code, whose loads of a next tile the last
+    // makes like that: with a copy of its own for the last tile short parts ran twice the code, most of it not in a cache.)
+    auto tile_of = [&](const void* pool, uint32_t page, uint32_t t, bool is) {
         const uint32_t r = ((sp.first + t) * 16) & ((1u << c.page_shift) - 1), no = page < c.n_pages ? page : 0u;
-        return Tile{paged_tile(pool, Q::row_at(c, no, kvh, r), 16 * ROW), paged_tile(pool, Q::meta_at(c, no, kvh, r), Q::META)};
+        return Tile{paged_tile(pool, Q::row_at(c, no, kvh, r), is ? 16 * ROW : 0),
+                    paged_tile(pool, Q::meta_at(c, no, kvh, r), is ? Q::META : 0)};
     };
     typename WordsOf<KW>::type k[KL];
     typename WordsOf<VW ? VW : 1>::type v[4][VN];  // rows 4 g4 .. 4 g4 + 3
@@ -157,11 +159,11 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
 
     // ---- the query rows into LDS: each head's scaled by a power of two and split into two fp16 parts, whose sum it
     // is to 2^-22; a piece is 8 dims of a head, in the order in which the tiles' whole numbers come out of their words ----
-    constexpr int PH = DH / 8, QP = (HR * PH + 255) / 256;  // pieces of a head, of a thread
+    constexpr int PH = DH / 8, QP = (HR * PH + 64 * W - 1) / (64 * W);  // pieces of a head, of a thread
     f4v qr[QP][2];
 #pragma unroll
     for (int i = 0; i < QP; ++i) {
-        const int x = tid + 256 * i, h = x / PH;
+        const int x = tid + 64 * W * i, h = x / PH;
         const bool is = h < (int)nh;
 #pragma unroll
         for (int y = 0; y < 2; ++y)
@@ -169,10 +171,9 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
                           : f4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
     uint32_t t = mine.from + w;
-    // (a wave without a tile loads the part's last again, and uses nothing of it)
-    uint32_t page = page_of(min(t, e - 1)), page_next = t + 4 < e ? page_of(t + 4) : 0u;
+    uint32_t page = page_of(min(t, e - 1)), page_next = t + W < e ? page_of(t + W) : 0u;
     {
-        const Tile kt = tile_of(c.k, page, min(t, e - 1)), vt = tile_of(c.v, page, min(t, e - 1));
+        const Tile kt = tile_of(c.k, page, min(t, e - 1), t < e), vt = tile_of(c.v, page, min(t, e - 1), t < e);
 #pragma unroll
         for (int j = 0; j < KL; ++j) load_k(kt, j, key, g4);
         load_ks(kt, key, g4);
@@ -180,8 +181,8 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     }
 #pragma unroll
     for (int i = 0; i < QP; ++i) {
-        const int x = tid + 256 * i, h = x / PH, ch = x % PH;
-        if (QP * 256 > HR * PH && x >= HR * PH) break;
+        const int x = tid + 64 * W * i, h = x / PH, ch = x % PH;
+        if (QP * 64 * W > HR * PH && x >= HR * PH) break;
         uint32_t big = 0;
 #pragma unroll
         for (int y = 0; y < 8; ++y) big = max(big, __float_as_uint(qr[i][y / 4][y % 4]) & 0x7FFFFFFFu);
@@ -215,7 +216,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     const bool lower = NHQ < 4 && key / HR % 2;
     const float qf = k_s[key % HR] * p.scale * (p.softcap > 0.0f ? 1.0f : LOG2E);
     float m = G4A_NEG_INF, l = 0.0f;
-    float rs = 0x1p110f;  // P V's power of two: 2^10 over the largest S of V so far, rounded down to one
+    float rs = 0x1p106f;  // P V's power of two: 2^6 over the largest S of V so far, rounded down to one
     f4v acc[NA];
 #pragma unroll
     for (int d = 0; d < NA; ++d) acc[d] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -226,22 +227,22 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
         if constexpr (DH == 512 && NHQ < 4) asm volatile("" : "+v"(x));
         return x;
     };
-    auto tile = [&](auto more) {
-        constexpr bool MORE = decltype(more)::value;
+    for (; t < e; t += W) {
         const int ln = lane_again(), g4 = ln >> 4, key = ln & 15;
-        const uint32_t page_after = MORE && t + 8 < e ? page_of(t + 8) : 0u;
-        const Tile kt = tile_of(c.k, MORE ? page_next : 0u, MORE ? t + 4 : t);
+        const bool more = t + W < e, first = t == mine.from + w;
+        const uint32_t page_after = t + 2 * W < e ? page_of(t + 2 * W) : 0u;
+        const Tile kt = tile_of(c.k, page_next, t + W, more);
         // ---- scores ----
         f4v d[NHQ == 4 ? 2 : 1];
 #pragma unroll
         for (int y = 0; y < (NHQ == 4 ? 2 : 1); ++y) d[y] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+        // (a row's columns are turned by its number modulo COLS: 4 mt and g4, which share no bit)
+        const f16x8* const qrow = qs + g4 * COLS;
+        const int col = (key ^ g4) % COLS;
         auto mac = [&](int mt, const f16x8& a) {
-            const int row = 4 * mt + g4;
 #pragma unroll
-            for (int y = 0; y < (NHQ == 4 ? 2 : 1); ++y) {
-                const int col = NHQ == 4 ? key + 16 * y : key % COLS;
-                d[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qs[row * COLS + (col ^ (row % COLS))], d[y], 0, 0, 0);
-            }
+            for (int y = 0; y < (NHQ == 4 ? 2 : 1); ++y)
+                d[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qrow[(col ^ ((4 * mt + 16 * y) % COLS)) + 4 * mt * COLS], d[y], 0, 0, 0);
         };
 #pragma unroll
         for (int j = 0; j < KL; ++j) {
@@ -261,7 +262,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
                                            byte_fields(two_bytes<0, 1>(k[j][i + 1], k[j][i + 1])),
                                            byte_fields(two_bytes<2, 3>(k[j][i + 1], k[j][i + 1]))}));
             }
-            if constexpr (MORE) load_k(kt, j, key, g4);
+            load_k(kt, j, key, g4);
             __builtin_amdgcn_sched_barrier(0);
         }
         f4v x;
@@ -288,7 +289,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
                 sv[r] = seen ? sv[r] : 0.0f;
             }
         }
-        if constexpr (MORE) load_ks(kt, key, g4);
+        load_ks(kt, key, g4);
         // ---- running maximum and sum, in powers of two ----
         const float mt = g4a_col_max4(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
         if (__ballot(mt > m + LAZY)) {
@@ -296,22 +297,24 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
             const float corr = m == G4A_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= corr;
+            if (!first)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {  // the lanes of a head hold its factor
-                const float f = NHQ > 1 ? __shfl(corr, 4 * (g4 % NHQ) + r) : g4a_lane(corr, r);
+                for (int r = 0; r < 4; ++r) {  // the lanes of a head hold its factor
+                    const float f = NHQ > 1 ? __shfl(corr, 4 * (g4 % NHQ) + r) : g4a_lane(corr, r);
 #pragma unroll
-                for (int a = 0; a < NA; ++a) acc[a][r] *= f;
-            }
+                    for (int a = 0; a < NA; ++a) acc[a][r] *= f;
+                }
         }
-        // V's scales times rs stay below 2^11, and with the probability, at most 2^LAZY, below 2^15 of fp16's 65504: a
-        // probability is held to 2^-22, or 2^-35 (half of fp16's smallest step, over 2^10) of one of 1 at the largest S
+        // V's scales times rs stay below 2^7, and with the probability, at most 2^LAZY, below 2^15 of fp16's 65504: a
+        // probability is held to 2^-22, or 2^-31 (half of fp16's smallest step, over 2^6) of one of 1 at the largest S
         const float top = fmaxf(fmaxf(fabsf(sv[0]), fabsf(sv[1])), fmaxf(fabsf(sv[2]), fabsf(sv[3])));
-        if (__ballot(top * rs >= 0x1p11f)) {
+        if (__ballot(top * rs >= 0x1p7f)) {
             const uint32_t r2 = __float_as_uint(g4a_col_max4(top)) & 0x7F800000u;
-            const float now = __uint_as_float((264u << 23) - r2), f = now / rs;
+            const float now = __uint_as_float((260u << 23) - r2), f = now / rs;
             rs = now;
+            if (!first)
 #pragma unroll
-            for (int a = 0; a < NA; ++a) acc[a] *= f;
+                for (int a = 0; a < NA; ++a) acc[a] *= f;
         }
         const float from = m == G4A_NEG_INF ? 0.0f : m;
         f4v pr;
@@ -334,7 +337,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
                 pa[0][r] = (_Float16)(lower ? y - (float)high : y);
             }
         }
-        const Tile vt = tile_of(c.v, MORE ? page_next : 0u, MORE ? t + 4 : t);
+        const Tile vt = tile_of(c.v, page_next, t + W, more);
         auto pv = [&](int a, uint32_t b0, uint32_t b1) {
             const f16x4 y = __builtin_bit_cast(f16x4, (typename WordsOf<2>::type){b0, b1});
 #pragma unroll
@@ -365,42 +368,53 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-        if constexpr (MORE) load_v(vt, key, g4);
+        load_v(vt, key, g4);
         page = page_next;
         page_next = page_after;
-    };
-    for (; t + 4 < e; t += 4) tile(std::true_type());
-    if (t < e) tile(std::false_type());
+    }
 
     // ---- the waves' partials, through LDS ----
     l = g4a_col_sum4(l);
     if (lane < HR) m_s[w][lane] = m, l_s[w][lane] = l;
     if (lane == 0) r_s[w] = (I4 ? 0x1p12f : 0x1p9f) / rs;
     barrier_lds();  // every wave is done with the query rows, where the accumulators go
+    if constexpr (NHQ == 4) {
 #pragma unroll
-    for (int d = 0; d < NA; ++d) {
-        if constexpr (NHQ < 4)  // the rows of a head's parts, in lanes 16 NHQ apart
+        for (int d = 0; d < NA; ++d) mrg[(w * NA + d) * 64 + lane] = acc[d];
+    } else {
+        // A head's two parts are in lanes 16 NHQ apart. Two accumulators at a time: a swap brings the first parts of both
+        // together, and the second parts, and the sums of the one are in the lower of these lanes, of the other in the upper.
+#pragma unroll
+        for (int d = 0; d < NA / 2; ++d) {
+            f4v y;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float2 y = NHQ == 2 ? g4a_pair32(acc[d][r]) : g4a_pair16(acc[d][r]);
-                acc[d][r] = y.x + y.y;
+                const uint32_t one = __float_as_uint(acc[d][r]), two = __float_as_uint(acc[d + NA / 2][r]);
+                if constexpr (NHQ == 2) {
+                    const auto z = __builtin_amdgcn_permlane32_swap(one, two, false, false);
+                    y[r] = __uint_as_float(z[0]) + __uint_as_float(z[1]);
+                } else {
+                    const auto z = __builtin_amdgcn_permlane16_swap(one, two, false, false);
+                    y[r] = __uint_as_float(z[0]) + __uint_as_float(z[1]);
+                }
             }
-        if (ML == 64 || lane < ML) mrg[(w * NA + d) * ML + lane] = acc[d];
+            if (lane < 2 * ML) mrg[(w * NA + d + lane / ML * (NA / 2)) * ML + lane % ML] = y;
+        }
     }
     const bool whole = mine.parts == 1;
     if (tid < HR) {
-        float M = G4A_NEG_INF, L = 0.0f, f[4];
+        float M = G4A_NEG_INF, L = 0.0f, f[W];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) M = fmaxf(M, m_s[i][tid]);
+        for (int i = 0; i < W; ++i) M = fmaxf(M, m_s[i][tid]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < W; ++i) {
             f[i] = m_s[i][tid] == G4A_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m_s[i][tid] - M);
             // (a sum without a maximum: scores that are NaN)
             L += m_s[i][tid] == G4A_NEG_INF ? l_s[i][tid] : l_s[i][tid] * f[i];
         }
         const float inv = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f_s[i][tid] = f[i] * inv * r_s[i];
+        for (int i = 0; i < W; ++i) f_s[i][tid] = f[i] * inv * r_s[i];
         if (!whole) {
             float* const ml = p.part_ml + (size_t)at * 2 * HR + tid;
             ml[0] = M;
@@ -409,11 +423,11 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     }
     barrier_lds();
     f4v* const dst = reinterpret_cast<f4v*>(p.part) + (size_t)at * C::ITEMS;
-    for (int i = tid; i < C::ITEMS; i += 256) {
+    for (int i = tid; i < C::ITEMS; i += 64 * W) {
         const int hq = C::hq(i), n = i % 16, a = i / 16 % NA;
         f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
+        for (int y = 0; y < W; ++y)
             o += mrg[(y * NA + a) * ML + 16 * hq + n] * *reinterpret_cast<const f4v*>(&f_s[y][4 * hq]);
         if (I4 && a % 2 == 0) o *= 16.0f;
         if (whole) {
@@ -430,10 +444,14 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
 }  // namespace
 
 #define G4A_PAGED_QUANT_DECODE(dh, type, bits, nhq, occ)                                                      \
-    extern "C" __global__ __launch_bounds__(256, occ) void g4a_paged_decode_d##dh##_##type##_h##nhq(          \
-        G4aPagedAttnParams p) { paged_decode_quant<dh, bits, nhq, false>(p); }                                \
-    extern "C" __global__ __launch_bounds__(256, occ) void g4a_paged_decode_win_d##dh##_##type##_h##nhq(      \
-        G4aPagedAttnParams p) { paged_decode_quant<dh, bits, nhq, true>(p); }                                 \
+    extern "C" __global__ __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), occ)                           \
+        void g4a_paged_decode_d##dh##_##type##_h##nhq(G4aPagedAttnParams p) {                                 \
+        paged_decode_quant<dh, bits, nhq, false>(p);                                                          \
+    }                                                                                                         \
+    extern "C" __global__ __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), occ)                           \
+        void g4a_paged_decode_win_d##dh##_##type##_h##nhq(G4aPagedAttnParams p) {                             \
+        paged_decode_quant<dh, bits, nhq, true>(p);                                                           \
+    }                                                                                                         \
     extern "C" __global__ __launch_bounds__(512) void g4a_paged_combine16_d##dh##_##type##_h##nhq(            \
         G4aPagedAttnParams p) { paged_combine<QuantCfg<dh, bits, nhq>, 16, 8>(p); }                           \
     extern "C" __global__ __launch_bounds__(256) void g4a_paged_combine64_d##dh##_##type##_h##nhq(            \
@@ -445,6 +463,6 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
 G4A_PAGED_QUANT_TYPES(64, 1, 4, 4) G4A_PAGED_QUANT_TYPES(64, 2, 4, 4) G4A_PAGED_QUANT_TYPES(64, 4, 4, 4)
 G4A_PAGED_QUANT_TYPES(128, 1, 4, 4) G4A_PAGED_QUANT_TYPES(128, 2, 4, 4) G4A_PAGED_QUANT_TYPES(128, 4, 4, 4)
 G4A_PAGED_QUANT_TYPES(256, 1, 3, 3) G4A_PAGED_QUANT_TYPES(256, 2, 3, 3) G4A_PAGED_QUANT_TYPES(256, 4, 2, 2)
-G4A_PAGED_QUANT_TYPES(512, 1, 2, 2) G4A_PAGED_QUANT_TYPES(512, 2, 2, 2) G4A_PAGED_QUANT_TYPES(512, 4, 1, 1)
+G4A_PAGED_QUANT_TYPES(512, 1, 1, 1) G4A_PAGED_QUANT_TYPES(512, 2, 1, 1) G4A_PAGED_QUANT_TYPES(512, 4, 1, 1)
 #undef G4A_PAGED_QUANT_TYPES
 #undef G4A_PAGED_QUANT_DECODE

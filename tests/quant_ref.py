@@ -106,9 +106,9 @@ def unpack(buf, dh, hkv, page, kv_type, vals):
 
 def attention(q, k, v, table, lens, *, scale=1.0, ring=False, **kw):
     """paged_ref.attention on the values of the pages, its bound widened by what the queries and probabilities of
-    two fp16 parts are off: 2^-22 of a value of a score's terms (|q||k| at most in all) and of a probability's, and 2^-35 of
+    two fp16 parts are off: 2^-22 of a value of a score's terms (|q||k| at most in all) and of a probability's, and 2^-31 of
     the largest value seen for each token: fp16 ends in steps of 2^-24, so a low part is off by 2^-25 at least, where a
-    weight e^(s - m) of 1 with the largest S seen stands at 2^10 and more, and the weights' sum is at least 1."""
+    weight e^(s - m) of 1 with the largest S seen stands at 2^6 and more, and the weights' sum is at least 1."""
     out, bound = ref.attention(q, k, v, table, lens, scale=scale, ring=ring, **kw)
     n, hq, dh = q.shape
     group = hq // k.shape[2]
@@ -128,5 +128,5 @@ def attention(q, k, v, table, lens, *, scale=1.0, ring=False, **kw):
             p = np.exp(s - s.max())
             p /= p.sum()
             score = 2.0 ** -22 * abs(scale) * np.linalg.norm(q[b, h]) * np.linalg.norm(kh, axis=1).max()
-            wide[b, h] += (2 * score + 2.0 ** -22) * (p @ np.abs(vh)) + 2.0 ** -35 * len(kh) * np.abs(vh).max()
+            wide[b, h] += (2 * score + 2.0 ** -22) * (p @ np.abs(vh)) + 2.0 ** -31 * len(kh) * np.abs(vh).max()
     return out, wide.reshape(bound.shape)
