@@ -142,13 +142,13 @@ __device__ __forceinline__ size_t uniform(size_t x) {
 }
 
 // This workgroup's part: tiles from .. to - 1 of sequence b's, one of `parts` of its unit of the query heads h0 .. h0 +
-// nh - 1 over kv head kvh. False where it has none. `lens`: LDS for PAGED_SEQS words.
+// nh - 1 over kv head kvh. False where it has none. `lens`: LDS for PAGED_SEQS words. ALL: every wave calls it, else one.
 struct PagedPart {
     PagedSpan sp;
     uint32_t b, parts, from, to, kvh, h0, nh;
 };
 
-template <int HR>
+template <int HR, bool ALL = true>
 __device__ __forceinline__ bool paged_find(const G4aPagedAttnParams& p, uint32_t* lens, int lane, int w, PagedPart& x) {
     // every wave sums the lengths, a span of `each` sequences a lane
     const uint32_t n = p.c.n_seqs, each = (n + 63) / 64;
@@ -198,7 +198,7 @@ __device__ __forceinline__ bool paged_find(const G4aPagedAttnParams& p, uint32_t
         base += __builtin_amdgcn_readlane(incl - mine_of, l1);
         x.b += l1;
         len = __builtin_amdgcn_readfirstlane(lens[x.b]);
-        barrier_lds();  // every wave has read the lengths: what comes next goes there
+        if constexpr (ALL) barrier_lds();  // every wave has read the lengths: what comes next goes there
     }
     x.sp = paged_span(p, len);
     x.parts = __builtin_amdgcn_readfirstlane(paged_parts(x.sp.n, quota));

@@ -89,6 +89,16 @@ __device__ __forceinline__ uint32_t byte_fields(uint32_t w) {
 }
 
 constexpr float LOG2E = 0x1.715476p+0f;
+
+// tanh to 2 units in the last place or so, in 14 instructions (tanhf is 46; with a soft-cap four of it were half of a
+// tile of 128 dims): below 1/2 z + z^3 P(z^2), P fitted to 2^-25 of the result there; else 1 - 2 / (e^2|z| + 1).
+__device__ __forceinline__ float quick_tanh(float z) {
+    const float u = z * z;
+    const float p = fmaf(fmaf(fmaf(0.0172569659f, u, -0.0530529357f), u, 0.133259878f), u, -0.333331496f);
+    const float e = __builtin_amdgcn_exp2f(2.0f * LOG2E * fabsf(z));
+    const float far = copysignf(fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), z);
+    return fabsf(z) < 0.5f ? fmaf(z * u, p, z) : far;
+}
 // Scores are relative to a maximum that follows the tiles' by more than this (of 2^x) alone: the accumulators are
 // scaled then, which took a fifth of a tile's vector instructions where every new maximum did.
 constexpr float LAZY = 8.0f;
@@ -103,14 +113,27 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     constexpr int VN = DH / (16 * EV), VBY = EV * BITS / 8, VW = VBY / 4;     // V: blocks of dims, a lane's bytes and words
     __shared__ __attribute__((aligned(16))) char smem[C::SM];
     __shared__ __attribute__((aligned(16))) float f_s[W][HR];
-    __shared__ float m_s[W][HR], l_s[W][HR], r_s[W], k_s[HR];
+    __shared__ float m_s[W][HR], l_s[W][HR], k_s[HR];
     f16x8* const qs = reinterpret_cast<f16x8*>(smem);
     f4v* const mrg = reinterpret_cast<f4v*>(smem);
     const G4aPaged& c = p.c;
     const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, key = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // (one wave looks its part up, for all: with 16 waves of a CU at it each, of 128 sequences, it took 4 us of a call)
+    __shared__ PagedPart found;
+    __shared__ bool any;
+    if (w == 0) {
+        PagedPart x;
+        const bool is = paged_find<HR, false>(p, reinterpret_cast<uint32_t*>(smem), lane, 0, x);
+        if (lane == 0) found = x, any = is;
+    }
+    barrier_lds();
+    if (!any) return;
     PagedPart mine;
-    if (!paged_find<HR>(p, reinterpret_cast<uint32_t*>(smem), lane, w, mine)) return;
+    static_assert(sizeof mine % 4 == 0, "words");
+#pragma unroll
+    for (int i = 0; i < (int)sizeof mine / 4; ++i)
+        reinterpret_cast<uint32_t*>(&mine)[i] = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(&found)[i]);
     const PagedSpan sp = mine.sp;
     const uint32_t at = blockIdx.x, b = mine.b, e = mine.to, h0 = mine.h0, nh = mine.nh, kvh = mine.kvh;
     if (sp.n == 0) {
@@ -173,11 +196,10 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     uint32_t t = mine.from + w;
     uint32_t page = page_of(min(t, e - 1)), page_next = t + W < e ? page_of(t + W) : 0u;
     {
-        const Tile kt = tile_of(c.k, page, min(t, e - 1), t < e), vt = tile_of(c.v, page, min(t, e - 1), t < e);
+        const Tile kt = tile_of(c.k, page, min(t, e - 1), t < e);
 #pragma unroll
         for (int j = 0; j < KL; ++j) load_k(kt, j, key, g4);
         load_ks(kt, key, g4);
-        load_v(vt, key, g4);
     }
 #pragma unroll
     for (int i = 0; i < QP; ++i) {
@@ -210,11 +232,13 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
         qs[row * COLS + (h ^ (row % COLS))] = hi;  // (the columns turned, or a wave's writes would meet in four banks)
         qs[row * COLS + ((HR + h) ^ (row % COLS))] = lo;
     }
+    load_v(tile_of(c.v, page, min(t, e - 1), t < e), key, g4);  // (ahead of the queries it would be ahead of other waves' too)
     barrier_lds();  // (K and V stay in flight across it)
 
     // lane (g4, n): keys 4 g4 + r of the tile, head n % HR of the unit; part n / HR % 2 of the queries and probabilities
     const bool lower = NHQ < 4 && key / HR % 2;
     const float qf = k_s[key % HR] * p.scale * (p.softcap > 0.0f ? 1.0f : LOG2E);
+    const float cap_inv = 1.0f / p.softcap;  // (where there is one)
     float m = G4A_NEG_INF, l = 0.0f;
     float rs = 0x1p106f;  // P V's power of two: 2^6 over the largest S of V so far, rounded down to one
     f4v acc[NA];
@@ -233,31 +257,41 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
         const uint32_t page_after = t + 2 * W < e ? page_of(t + 2 * W) : 0u;
         const Tile kt = tile_of(c.k, page_next, t + W, more);
         // ---- scores ----
-        f4v d[NHQ == 4 ? 2 : 1];
+        constexpr int KM = I4 ? KW : 2, QN = NHQ == 4 ? 2 : 1;  // MFMA steps of a load; query operands of a step
+        f4v d[QN];
 #pragma unroll
-        for (int y = 0; y < (NHQ == 4 ? 2 : 1); ++y) d[y] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int y = 0; y < QN; ++y) d[y] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
         // (a row's columns are turned by its number modulo COLS: 4 mt and g4, which share no bit)
         const f16x8* const qrow = qs + g4 * COLS;
         const int col = (key ^ g4) % COLS;
-        auto mac = [&](int mt, const f16x8& a) {
+        f16x8 qb[2][KM][QN];  // those of a load's steps are read ahead of the load before it
+        auto read_q = [&](int j) {
 #pragma unroll
-            for (int y = 0; y < (NHQ == 4 ? 2 : 1); ++y)
-                d[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qrow[(col ^ ((4 * mt + 16 * y) % COLS)) + 4 * mt * COLS], d[y], 0, 0, 0);
+            for (int i = 0; i < KM; ++i)
+#pragma unroll
+                for (int y = 0; y < QN; ++y)
+                    qb[j % 2][i][y] = qrow[(col ^ ((4 * (KM * j + i) + 16 * y) % COLS)) + 4 * (KM * j + i) * COLS];
         };
+        auto mac = [&](int j, int i, const f16x8& a) {
+#pragma unroll
+            for (int y = 0; y < QN; ++y) d[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qb[j % 2][i][y], d[y], 0, 0, 0);
+        };
+        read_q(0);
 #pragma unroll
         for (int j = 0; j < KL; ++j) {
+            if (j + 1 < KL) read_q(j + 1);
             if constexpr (I4) {
                 const SubPair s = sub_pair(ksub, j | j << 16);
 #pragma unroll
                 for (int i = 0; i < KW; ++i) {
                     const uint32_t x = k[j][i], y = x >> 8;
-                    mac(KW * j + i, __builtin_bit_cast(f16x8, (typename WordsOf<4>::type){low_fields(x, s), high_fields(x, s),
+                    mac(j, i, __builtin_bit_cast(f16x8, (typename WordsOf<4>::type){low_fields(x, s), high_fields(x, s),
                                                                                            low_fields(y, s), high_fields(y, s)}));
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; i += 2)
-                    mac(2 * j + i / 2, __builtin_bit_cast(f16x8, (typename WordsOf<4>::type){
+                    mac(j, i / 2, __builtin_bit_cast(f16x8, (typename WordsOf<4>::type){
                                            byte_fields(two_bytes<0, 1>(k[j][i], k[j][i])), byte_fields(two_bytes<2, 3>(k[j][i], k[j][i])),
                                            byte_fields(two_bytes<0, 1>(k[j][i + 1], k[j][i + 1])),
                                            byte_fields(two_bytes<2, 3>(k[j][i + 1], k[j][i + 1]))}));
@@ -273,7 +307,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
             else x[r] = d[0][r] + g4a_dpp<ROW_ROR4>(d[0][r]);
             const float s = __uint_as_float(r % 2 ? ks[r / 2] & 0xFFFF0000u : ks[r / 2] << 16);
             x[r] *= s * 0x1p6f * qf;
-            if (p.softcap > 0.0f) x[r] = p.softcap * LOG2E * tanhf(x[r] / p.softcap);
+            if (p.softcap > 0.0f) x[r] = p.softcap * LOG2E * quick_tanh(x[r] * cap_inv);
         }
         f4v sv;
 #pragma unroll
@@ -322,7 +356,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
         for (int r = 0; r < 4; ++r) pr[r] = __builtin_amdgcn_exp2f(x[r] - from);
         l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
         // ---- P V: P is the A operand as it stands, in two parts ----
-        f16x4 pa[NHQ == 4 ? 2 : 1];
+        f16x4 pa[QN];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             float y = pr[r] * (sv[r] * rs);
@@ -341,7 +375,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
         auto pv = [&](int a, uint32_t b0, uint32_t b1) {
             const f16x4 y = __builtin_bit_cast(f16x4, (typename WordsOf<2>::type){b0, b1});
 #pragma unroll
-            for (int z = 0; z < (NHQ == 4 ? 2 : 1); ++z) acc[a] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa[z], y, acc[a], 0, 0, 0);
+            for (int z = 0; z < QN; ++z) acc[a] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa[z], y, acc[a], 0, 0, 0);
         };
         SubPair s01, s23;
         if constexpr (I4) s01 = sub_pair(vsub, 0x00010000u), s23 = sub_pair(vsub, 0x00030002u);
@@ -376,8 +410,23 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     // ---- the waves' partials, through LDS ----
     l = g4a_col_sum4(l);
     if (lane < HR) m_s[w][lane] = m, l_s[w][lane] = l;
-    if (lane == 0) r_s[w] = (I4 ? 0x1p12f : 0x1p9f) / rs;
     barrier_lds();  // every wave is done with the query rows, where the accumulators go
+    const bool whole = mine.parts == 1;
+    if (lane < HR) {  // this wave's factor of each head; all waves compute the heads' maximum and sum alike
+        float M = G4A_NEG_INF, L = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) M = fmaxf(M, m_s[i][lane]);
+#pragma unroll
+        for (int i = 0; i < W; ++i)  // (a sum without a maximum: scores that are NaN)
+            L += m_s[i][lane] == G4A_NEG_INF ? l_s[i][lane] : l_s[i][lane] * __builtin_amdgcn_exp2f(m_s[i][lane] - M);
+        const float f = (m == G4A_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m - M)) * ((I4 ? 0x1p12f : 0x1p9f) / rs);
+        f_s[w][lane] = whole ? f * (L != 0.0f ? 1.0f / L : 0.0f) : f;
+        if (!whole && w == 0) {
+            float* const ml = p.part_ml + (size_t)at * 2 * HR + lane;
+            ml[0] = M;
+            ml[HR] = L;
+        }
+    }
     if constexpr (NHQ == 4) {
 #pragma unroll
         for (int d = 0; d < NA; ++d) mrg[(w * NA + d) * 64 + lane] = acc[d];
@@ -401,29 +450,12 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
             if (lane < 2 * ML) mrg[(w * NA + d + lane / ML * (NA / 2)) * ML + lane % ML] = y;
         }
     }
-    const bool whole = mine.parts == 1;
-    if (tid < HR) {
-        float M = G4A_NEG_INF, L = 0.0f, f[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) M = fmaxf(M, m_s[i][tid]);
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            f[i] = m_s[i][tid] == G4A_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m_s[i][tid] - M);
-            // (a sum without a maximum: scores that are NaN)
-            L += m_s[i][tid] == G4A_NEG_INF ? l_s[i][tid] : l_s[i][tid] * f[i];
-        }
-        const float inv = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) f_s[i][tid] = f[i] * inv * r_s[i];
-        if (!whole) {
-            float* const ml = p.part_ml + (size_t)at * 2 * HR + tid;
-            ml[0] = M;
-            ml[HR] = L;
-        }
-    }
     barrier_lds();
     f4v* const dst = reinterpret_cast<f4v*>(p.part) + (size_t)at * C::ITEMS;
-    for (int i = tid; i < C::ITEMS; i += 64 * W) {
+#pragma unroll
+    for (int i0 = 0; i0 < C::ITEMS; i0 += 64 * W) {
+        const int i = i0 + tid;
+        if (C::ITEMS % (64 * W) && i >= C::ITEMS) break;
         const int hq = C::hq(i), n = i % 16, a = i / 16 % NA;
         f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
