@@ -2366,8 +2366,8 @@ constexpr uint32_t PAGED_UNITS = 2048;
 // [head_dim 64, 128, 256, 512][f32, bf16, 8-bit, 4-bit pages][4, 8, 16 heads a unit].
 constexpr uint32_t PAGED_WGS_PER_CU[4][4][3] = {
     {{4, 4, 2}, {4, 4, 4}, {4, 4, 4}, {4, 4, 4}},
-    {{3, 3, 2}, {4, 4, 3}, {4, 4, 3}, {4, 4, 3}},
-    {{2, 2, 1}, {3, 3, 2}, {3, 3, 2}, {3, 3, 2}},
+    {{3, 3, 2}, {4, 4, 3}, {3, 4, 2}, {3, 4, 2}},
+    {{2, 2, 1}, {3, 3, 2}, {1, 1, 1}, {1, 1, 1}},
     {{1, 1, 1}, {1, 1, 1}, {1, 1, 1}, {1, 1, 1}}};
 
 // Index of a paged cache's head_dim among the kernels'.
@@ -2560,8 +2560,8 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     if (std::max<uint64_t>(p.span / 16 + 2, item / 64) * cache->n_seqs * p.units >> 31)
         return fail(ctx, G4A_E_SHAPE, "%u sequences of up to %u tokens in %u head groups: at most 2^31 tiles of 16 tokens",
                     cache->n_seqs, p.span, p.units);
-    // (8 and 4 bits of 512 dims and up to 8 heads: eight waves, attn_paged_quant.hip)
-    const uint32_t waves = paged_quant(cache->kv_type) && cache->Dh == 512 && h < 2 ? 8 : 4;
+    const bool quant = paged_quant(cache->kv_type);
+    const uint32_t waves = quant ? g4a_paged_waves(int(cache->Dh), 1 << h) : 4;
     p.min_part = std::max(PAGED_MIN_PART, waves);
     p.scale = a->scale;
     p.softcap = a->attn_softcap;
@@ -2571,7 +2571,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     // second workgroup that a CU has room for takes (256 sequences of up to 1500 tokens, f32: 114 us with them,
     // 143 without, 127 with as many again; bf16 69, 82, 79; 100 of up to 4000, where there are fewer units, are not
     // concerned).
-    const uint32_t over = d == 3 && h < 2 ? resident + resident / 2 : resident;
+    const uint32_t over = quant ? (d == 2 ? 3 * resident : resident) : d == 3 && h < 2 ? resident + resident / 2 : resident;
     // launches of at most PAGED_UNITS units, which bounds the partials' memory, and of as many sequences as
     // the kernel counts
     const uint32_t most = std::min({cache->n_seqs, std::max(1u, PAGED_UNITS / p.units), PAGED_SEQS});

@@ -20,7 +20,7 @@ struct QuantCfg {
     static constexpr int NA = DH / 16;                                // accumulators of a lane, of 16 rows
     static constexpr int ITEMS = NHQ * DH;                            // (4 heads, dim) of a partial
     static constexpr int ML = 16 * NHQ;                               // lanes with a row of heads each, per accumulator
-    static constexpr int W = DH == 512 && NHQ < 4 ? 8 : 4;            // waves
+    static constexpr int W = g4a_paged_waves(DH, NHQ);                // waves
     // the queries (two fp16 parts), the waves' accumulators and the sequences' lengths never live at once
     static constexpr int SM0 = 4 * HR * DH > W * NA * ML * 16 ? 4 * HR * DH : W * NA * ML * 16;
     static constexpr int SM = SM0 > 4096 ? SM0 : 4096;
@@ -476,11 +476,11 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
 }  // namespace
 
 #define G4A_PAGED_QUANT_DECODE(dh, type, bits, nhq, occ)                                                      \
-    extern "C" __global__ __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), occ)                           \
+    extern "C" __global__ __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), (occ * QuantCfg<dh, bits, nhq>::W / 4))                           \
         void g4a_paged_decode_d##dh##_##type##_h##nhq(G4aPagedAttnParams p) {                                 \
         paged_decode_quant<dh, bits, nhq, false>(p);                                                          \
     }                                                                                                         \
-    extern "C" __global__ __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), occ)                           \
+    extern "C" __global__ __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), (occ * QuantCfg<dh, bits, nhq>::W / 4))                           \
         void g4a_paged_decode_win_d##dh##_##type##_h##nhq(G4aPagedAttnParams p) {                             \
         paged_decode_quant<dh, bits, nhq, true>(p);                                                           \
     }                                                                                                         \
