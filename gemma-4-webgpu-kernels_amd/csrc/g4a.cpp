@@ -2423,13 +2423,11 @@ int paged_cache(g4a_ctx* ctx, const g4a_paged_cache* c, bool tables, bool pools,
     return G4A_OK;
 }
 
-// Launches a kernel on T * Hkv rows of K and as many of V: a wave takes `turns` lots of them, one after the other.
-int paged_rows(g4a_ctx* ctx, const g4a_paged_cache* c, hipFunction_t (&kernels)[4][4], G4aPagedRowsParams& p,
+// Launches a kernel on T * Hkv rows of K and as many of V.
+int paged_rows(g4a_ctx* ctx, const g4a_paged_cache* c, hipFunction_t (&kernels)[4][4], const G4aPagedRowsParams& p,
                const char* what) {
     const uint32_t at_once = std::max<uint32_t>(1, 256 / c->Dh);  // rows a wave holds
-    const uint64_t rows = uint64_t(p.T) * c->Hkv;
-    p.turns = 1;
-    const uint64_t wgs = (rows + 4 * p.turns * at_once - 1) / (4 * p.turns * at_once);
+    const uint64_t rows = uint64_t(p.T) * c->Hkv, wgs = (rows + 4 * at_once - 1) / (4 * at_once);
     if (wgs > PAGED_GRID) return fail(ctx, G4A_E_SHAPE, "too many rows (%llu)", (unsigned long long)rows);
     return launch(ctx, kernels[paged_dh(c->Dh)][paged_type(c->kv_type)], dim3(uint32_t(wgs), 2, 1), dim3(256, 1, 1), p, what,
                   true);

@@ -113,7 +113,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     constexpr int VN = DH / (16 * EV), VBY = EV * BITS / 8, VW = VBY / 4;     // V: blocks of dims, a lane's bytes and words
     __shared__ __attribute__((aligned(16))) char smem[C::SM];
     __shared__ __attribute__((aligned(16))) float f_s[W][HR];
-    __shared__ float m_s[W][HR], l_s[W][HR], k_s[HR];
+    __shared__ float m_s[W][HR], l_s[W][HR], r_s[W], k_s[HR];
     f16x8* const qs = reinterpret_cast<f16x8*>(smem);
     f4v* const mrg = reinterpret_cast<f4v*>(smem);
     const G4aPaged& c = p.c;
@@ -410,22 +410,33 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     // ---- the waves' partials, through LDS ----
     l = g4a_col_sum4(l);
     if (lane < HR) m_s[w][lane] = m, l_s[w][lane] = l;
+    if (lane == 0) r_s[w] = (I4 ? 0x1p12f : 0x1p9f) / rs;
     barrier_lds();  // every wave is done with the query rows, where the accumulators go
     const bool whole = mine.parts == 1;
-    if (lane < HR) {  // this wave's factor of each head; all waves compute the heads' maximum and sum alike
-        float M = G4A_NEG_INF, L = 0.0f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) M = fmaxf(M, m_s[i][lane]);
-#pragma unroll
-        for (int i = 0; i < W; ++i)  // (a sum without a maximum: scores that are NaN)
-            L += m_s[i][lane] == G4A_NEG_INF ? l_s[i][lane] : l_s[i][lane] * __builtin_amdgcn_exp2f(m_s[i][lane] - M);
-        const float f = (m == G4A_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m - M)) * ((I4 ? 0x1p12f : 0x1p9f) / rs);
-        f_s[w][lane] = whole ? f * (L != 0.0f ? 1.0f / L : 0.0f) : f;
-        if (!whole && w == 0) {
+    if (w == 0) {  // the waves' factors of each head: lane HR i + h for wave i and head h
+        const int i = lane / HR, h = lane % HR;
+        const bool is = i < W;
+        const float mi = is ? m_s[i][h] : G4A_NEG_INF, li = is ? l_s[i][h] : 0.0f;
+        auto over_waves = [&](float x, auto op) {  // the lanes of a head are HR apart
+            if constexpr (HR == 4) x = op(x, g4a_dpp<ROW_ROR4>(x));
+            if constexpr (HR <= 8) x = op(x, g4a_dpp<ROW_ROR8>(x));
+            float2 y = g4a_pair16(x);
+            x = op(y.x, y.y);
+            y = g4a_pair32(x);
+            return op(y.x, y.y);
+        };
+        static_assert(W * HR <= 64, "a lane a wave and head");
+        const float M = over_waves(mi, [](float a, float b) { return fmaxf(a, b); });
+        float f = mi == G4A_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
+        // (a sum without a maximum: scores that are NaN)
+        const float L = over_waves(mi == G4A_NEG_INF ? li : li * f, [](float a, float b) { return a + b; });
+        if (!whole && lane < HR) {
             float* const ml = p.part_ml + (size_t)at * 2 * HR + lane;
             ml[0] = M;
             ml[HR] = L;
         }
+        if (whole) f *= L != 0.0f ? 1.0f / L : 0.0f;
+        if (is) f_s[i][h] = f * r_s[i];
     }
     if constexpr (NHQ == 4) {
 #pragma unroll
@@ -460,7 +471,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
         f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int y = 0; y < W; ++y)
-            o += mrg[(y * NA + a) * ML + 16 * hq + n] * *reinterpret_cast<const f4v*>(&f_s[y][4 * hq]);
+            o = __builtin_elementwise_fma(mrg[(y * NA + a) * ML + 16 * hq + n], *reinterpret_cast<const f4v*>(&f_s[y][4 * hq]), o);
         if (I4 && a % 2 == 0) o *= 16.0f;
         if (whole) {
             const int dim = C::dim(i);

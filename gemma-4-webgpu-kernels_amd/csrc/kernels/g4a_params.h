@@ -404,7 +404,6 @@ struct G4aPagedRowsParams {
     const uint32_t* slots;   // device [T], or null: tokens pos0 .. of sequence seq
     uint32_t seq, pos0;
     uint32_t T;
-    uint32_t turns;          // of a wave, one after the other
 };
 
 // The producer into pages of 8 and 4 bits (g4a_paged_producer_d*_{i8,i4}): workgroups below q_wgs take the query rows,

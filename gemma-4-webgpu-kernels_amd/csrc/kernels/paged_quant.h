@@ -75,23 +75,36 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x) {
     return x;
 }
 
-// S of a row whose largest magnitude is `big` (finite).
+// S of a row whose largest magnitude is `big` (finite): about big / MOST, rounded up to a bfloat16, is it or next to
+// it, and MOST S is exact. (Divisions by rule of IEEE were half of a row's instructions, here and below.)
 template <int MOST>
 __device__ __forceinline__ float quant_scale(float big) {
-    const float t = fmaxf(big / (float)MOST, 0x1p-126f);
-    float s = __uint_as_float((__float_as_uint(t) + 0xFFFFu) & 0xFFFF0000u);
-    // (the quotient may have been rounded down onto a bfloat16; MOST S is exact)
-    if (s * (float)MOST < big) s = __uint_as_float(__float_as_uint(s) + 0x10000u);
-    return s;
+    const float t = fmaxf(big * (1.0f / MOST), 0x1p-126f);
+    const uint32_t up = (__float_as_uint(t) + 0xFFFFu) & 0xFFFF0000u;
+    const float s = __uint_as_float(up), less = fmaxf(__uint_as_float(up - 0x10000u), 0x1p-126f);
+    if (s * (float)MOST < big) return __uint_as_float(up + 0x10000u);
+    return less * (float)MOST >= big ? less : s;
 }
 
-// x / step rounded to nearest, halves to even, exactly: x * inv is at most a little off, x - n step is
-// exact (it has no more bits than x), and half the step too.
-__device__ __forceinline__ float quant_round(float x, float step, float inv) {
-    const float n = rintf(x * inv), r = fmaf(-n, step, x), half = 0.5f * fabsf(step);
-    const float away = (r < 0.0f) != (step < 0.0f) ? -1.0f : 1.0f;  // towards x
-    const bool odd = (int)n & 1;
-    return fabsf(r) > half || (fabsf(r) == half && odd) ? n + away : n;
+// x / step rounded to nearest, halves to even, exactly, for four values: x * inv (inv about 1 / step) rounds to it or next
+// to it, and x - n step, exact as it has no more bits than x, says which. That n is not x * inv's, or that x is
+// half way between two, is rare and looked for once.
+__device__ __forceinline__ f32x4 quant_round(const f32x4& x, float step, float inv) {
+    const float half = 0.5f * fabsf(step);
+    f32x4 n, r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        n[i] = rintf(x[i] * inv);
+        r[i] = fmaf(-n[i], step, x[i]);
+    }
+    if (__ballot(fmaxf(fmaxf(fabsf(r[0]), fabsf(r[1])), fmaxf(fabsf(r[2]), fabsf(r[3]))) >= half))
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float towards = (r[i] < 0.0f) != (step < 0.0f) ? -1.0f : 1.0f;
+            const bool odd = (int)n[i] & 1;
+            if (fabsf(r[i]) > half || (fabsf(r[i]) == half && odd)) n[i] += towards;
+        }
+    return n;
 }
 
 // A row into its place, by LPR lanes of which lane l holds dims 4 l .. and, at 512, 256 + 4 l ..; `is`: there is one.
@@ -117,22 +130,23 @@ __device__ __forceinline__ void quant_store(const G4aPaged& c, void* pool, uint3
         f32x4 y = x[e];
         if (bad) y = f32x4{0, 0, 0, 0};
         if constexpr (BITS == 8) {
-            const float inv = 1.0f / s;
-            uint32_t w = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w |= (uint32_t)(int)(quant_round(y[i], s, inv) + 128.0f) << (8 * i);
+            const f32x4 n = quant_round(y, s, __builtin_amdgcn_rcpf(s));
+            const uint32_t w = (uint32_t)fmaf(n[1], 256.0f, n[0] + 128.0f * 257.0f) |
+                               (uint32_t)fmaf(n[3], 256.0f, n[2] + 128.0f * 257.0f) << 16;
             if (is) *reinterpret_cast<uint32_t*>(row + 4 * l + 256 * e) = w;
         } else {
             const float high = g4a_max8(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
             const float low = g4a_max8(fmaxf(fmaxf(-y[0], -y[1]), fmaxf(-y[2], -y[3])));
             const float most = fmaxf(high, low);
-            float n = fmaxf(ceilf(most / (8.0f * s)), 1.0f);
-            if (n * (8.0f * s) < most) n += 1.0f;
-            const float sub = high >= low ? -n : n, step = s * sub, inv = 1.0f / step;
-            uint32_t w = 0;
+            const float s8 = 8.0f * s;
+            float c8 = fmaxf(ceilf(most * __builtin_amdgcn_rcpf(s8)), 1.0f);  // (or next to it; the products are exact)
+            if (c8 * s8 < most) c8 += 1.0f;
+            else if (c8 > 1.0f && (c8 - 1.0f) * s8 >= most) c8 -= 1.0f;
+            const float sub = high >= low ? -c8 : c8, step = s * sub;
+            f32x4 n = quant_round(y, step, __builtin_amdgcn_rcpf(step));
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                w |= (uint32_t)(int)(fminf(fmaxf(quant_round(y[i], step, inv), -8.0f), 7.0f) + 8.0f) << (4 * i);
+            for (int i = 0; i < 4; ++i) n[i] = fminf(fmaxf(n[i], -8.0f), 7.0f);
+            uint32_t w = (uint32_t)fmaf(n[3], 4096.0f, fmaf(n[2], 256.0f, fmaf(n[1], 16.0f, n[0] + 8.0f * 4369.0f)));
             w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, G4A_DPP_XOR1, 0xf, 0xf, false) << 16;
             if (is && l % 2 == 0) *reinterpret_cast<uint32_t*>(row + 2 * l + 128 * e) = w;
             if (is && l % 8 == 0) meta[Q::template sub_at<VALUES>((4 * l + 256 * e) / 32, r)] = (uint8_t)((int)sub + 128);

@@ -58,19 +58,16 @@ __device__ __forceinline__ void paged_write(const G4aPagedRowsParams& p) {
     using R = RowLanes<DH>;
     const G4aPaged& c = p.c;
     const int lane = threadIdx.x & 63, g = lane / R::LPR, l = lane % R::LPR;
-    const uint32_t rows = p.T * c.Hkv, first = (blockIdx.x * 4 + threadIdx.x / 64) * p.turns * R::RPW;
-    for (uint32_t i = 0; i < p.turns; ++i) {
-        const uint32_t row = first + i * R::RPW + g;
-        const bool is = row < rows;
-        const uint32_t t = is ? row / c.Hkv : 0u, slot = p.slots[t];
-        f32x4 x[R::E];
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t rows = p.T * c.Hkv, row = (blockIdx.x * 4 + w) * R::RPW + g;
+    const bool is = row < rows;
+    const uint32_t t = is ? row / c.Hkv : 0u, slot = p.slots[t];
+    f32x4 x[R::E];
 #pragma unroll
-        for (int e = 0; e < R::E; ++e)
-            x[e] = is ? *reinterpret_cast<const f32x4*>((VALUES ? p.v_in : p.k_in) + (size_t)row * DH + 4 * l + 256 * e)
-                      : f32x4{0, 0, 0, 0};
-        store_row<DH, BITS, VALUES>(c, VALUES ? c.v : c.k, slot, row - t * c.Hkv, l, x,
-                                    is && (slot >> c.page_shift) < c.n_pages);
-    }
+    for (int e = 0; e < R::E; ++e)
+        x[e] = is ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>((VALUES ? p.v_in : p.k_in) + (size_t)row * DH + 4 * l + 256 * e))
+                  : f32x4{0, 0, 0, 0};
+    store_row<DH, BITS, VALUES>(c, VALUES ? c.v : c.k, slot, row - t * c.Hkv, l, x, is && (slot >> c.page_shift) < c.n_pages);
 }
 
 // The slot of token t of a call: given, or that of position pos0 + t of its sequence; G4A_NO_ROW32 where the cache
@@ -89,25 +86,25 @@ __device__ __forceinline__ uint32_t paged_slot(const G4aPagedRowsParams& p, uint
     return page < c.n_pages ? (page << c.page_shift) + (pos & ((1u << c.page_shift) - 1)) : G4A_NO_ROW32;
 }
 
-// T tokens' rows as f32, zeros for those that the cache does not hold.
+// T tokens' rows as f32, zeros for those that the cache does not hold. The rows go past the caches: 32768 tokens of 512
+// dims in 4 bits take 23.3 us (6.5 TB/s read and written), 37.4 with plain stores. (Four rows a wave, their loads side by
+// side, 24.5.)
 template <int DH, int BITS, bool VALUES>
 __device__ __forceinline__ void paged_read(const G4aPagedRowsParams& p) {
     using R = RowLanes<DH>;
     const G4aPaged& c = p.c;
     const int lane = threadIdx.x & 63, g = lane / R::LPR, l = lane % R::LPR;
-    const uint32_t rows = p.T * c.Hkv, first = (blockIdx.x * 4 + threadIdx.x / 64) * p.turns * R::RPW;
-    for (uint32_t i = 0; i < p.turns; ++i) {
-        const uint32_t row = first + i * R::RPW + g;
-        if (row >= rows) return;
-        const uint32_t t = row / c.Hkv, slot = paged_slot(p, t);
-        f32x4 x[R::E];
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t rows = p.T * c.Hkv, row = (blockIdx.x * 4 + w) * R::RPW + g;
+    if (row >= rows) return;
+    const uint32_t t = row / c.Hkv, slot = paged_slot(p, t);
+    f32x4 x[R::E];
 #pragma unroll
-        for (int e = 0; e < R::E; ++e) x[e] = f32x4{0, 0, 0, 0};
-        if (slot != G4A_NO_ROW32) load_row<DH, BITS, VALUES>(c, VALUES ? c.v : c.k, slot, row - t * c.Hkv, l, x);
+    for (int e = 0; e < R::E; ++e) x[e] = f32x4{0, 0, 0, 0};
+    if (slot != G4A_NO_ROW32) load_row<DH, BITS, VALUES>(c, VALUES ? c.v : c.k, slot, row - t * c.Hkv, l, x);
 #pragma unroll
-        for (int e = 0; e < R::E; ++e)
-            *reinterpret_cast<f32x4*>((VALUES ? p.v_out : p.k_out) + (size_t)row * DH + 4 * l + 256 * e) = x[e];
-    }
+    for (int e = 0; e < R::E; ++e)
+        __builtin_nontemporal_store(x[e], reinterpret_cast<f32x4*>((VALUES ? p.v_out : p.k_out) + (size_t)row * DH + 4 * l + 256 * e));
 }
 
 // The K and V rows of the producer into pages of 8 and 4 bits: y = rope(x / sqrt(mean(x^2) + eps) * w) in 64 bits,
