@@ -156,6 +156,7 @@ struct g4a_ctx {
     hipFunction_t page_map[2] = {};  // [256, 1024 threads]
     hipFunction_t paged_producer[4][4] = {};
     hipFunction_t paged_decode[2][4][4][3] = {};  // [whole context, window] ... [4, 8, 16 heads a unit]
+    hipFunction_t paged_decode_many[2][2][2] = {};  // 512 dims, many units: [..][8-bit, 4-bit][4, 8 heads]
     hipFunction_t paged_combine[2][4][4][3] = {};  // [16, 64 items a block] ...
     hipFunction_t paged_gather[2] = {};            // f32 and bf16 pages, any head_dim
     hipFunction_t paged_write[4][4] = {};
@@ -935,6 +936,9 @@ int g4a_create_with(int device, const char* hsaco_path, const g4a_options* opts,
                 for (int win = 0; win < 2; ++win) {
                     snprintf(name, sizeof name, "g4a_paged_decode%s_d%d_%s_h%d", win ? "_win" : "", 64 << d, types[t], 1 << h);
                     if (int rc = get_fn(ctx, &ctx->paged_decode[win][d][t][h], name)) return bail(rc);
+                    if (t < 2 || d < 3 || h == 2) continue;
+                    snprintf(name, sizeof name, "g4a_paged_decode_many%s_d512_%s_h%d", win ? "_win" : "", types[t], 1 << h);
+                    if (int rc = get_fn(ctx, &ctx->paged_decode_many[win][t - 2][h], name)) return bail(rc);
                 }
                 for (int w = 0; w < 2; ++w) {
                     snprintf(name, sizeof name, "g4a_paged_combine%d_d%d_%s_h%d", w ? 64 : 16, 64 << d, types[t], 1 << h);
@@ -2559,7 +2563,8 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
         return fail(ctx, G4A_E_SHAPE, "%u sequences of up to %u tokens in %u head groups: at most 2^31 tiles of 16 tokens",
                     cache->n_seqs, p.span, p.units);
     const bool quant = paged_quant(cache->kv_type);
-    const uint32_t waves = quant ? g4a_paged_waves(int(cache->Dh), 1 << h) : 4;
+    const bool many = quant && cache->Dh == 512 && h < 2 && uint64_t(cache->n_seqs) * p.units >= uint32_t(std::max(ctx->cu_count, 1));
+    const uint32_t waves = quant ? g4a_paged_waves(int(cache->Dh), 1 << h, many) : 4;
     p.min_part = std::max(PAGED_MIN_PART, waves);
     p.scale = a->scale;
     p.softcap = a->attn_softcap;
@@ -2569,7 +2574,7 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     // second workgroup that a CU has room for takes (256 sequences of up to 1500 tokens, f32: 114 us with them,
     // 143 without, 127 with as many again; bf16 69, 82, 79; 100 of up to 4000, where there are fewer units, are not
     // concerned).
-    const uint32_t over = quant ? (d == 2 ? 3 * resident : resident) : d == 3 && h < 2 ? resident + resident / 2 : resident;
+    const uint32_t over = quant && d == 2 ? 3 * resident : (quant ? many : d == 3 && h < 2) ? resident + resident / 2 : resident;
     // launches of at most PAGED_UNITS units, which bounds the partials' memory, and of as many sequences as
     // the kernel counts
     const uint32_t most = std::min({cache->n_seqs, std::max(1u, PAGED_UNITS / p.units), PAGED_SEQS});
@@ -2602,7 +2607,8 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
         p.q = all.q + size_t(b0) * a->Hq * cache->Dh;
         p.out = all.out + size_t(b0) * a->Hq * cache->Dh;
         const uint32_t wgs = shares(p.c.n_seqs, &p.spread, &p.fit), units = p.c.n_seqs * p.units;
-        if (int rc = launch(ctx, ctx->paged_decode[a->sliding_window != 0][d][t][h], dim3(wgs, 1, 1), dim3(64 * waves, 1, 1), p,
+        const int win = a->sliding_window != 0;
+        if (int rc = launch(ctx, many ? ctx->paged_decode_many[win][t - 2][h] : ctx->paged_decode[win][d][t][h], dim3(wgs, 1, 1), dim3(64 * waves, 1, 1), p,
                             "paged decode", true))
             return rc;
         if (!splits) continue;

@@ -11,7 +11,7 @@
 
 namespace {
 
-template <int DH, int BITS, int NHQ>
+template <int DH, int BITS, int NHQ, bool MANY = false>
 struct QuantCfg {
     static constexpr int DIMS = DH;
     static __device__ __forceinline__ float exp(float x) { return __builtin_amdgcn_exp2f(x); }  // of the partials' maxima
@@ -20,7 +20,7 @@ struct QuantCfg {
     static constexpr int NA = DH / 16;                                // accumulators of a lane, of 16 rows
     static constexpr int ITEMS = NHQ * DH;                            // (4 heads, dim) of a partial
     static constexpr int ML = 16 * NHQ;                               // lanes with a row of heads each, per accumulator
-    static constexpr int W = g4a_paged_waves(DH, NHQ);                // waves
+    static constexpr int W = g4a_paged_waves(DH, NHQ, MANY);          // waves
     // the queries (two fp16 parts), the waves' accumulators and the sequences' lengths never live at once
     static constexpr int SM0 = 4 * HR * DH > W * NA * ML * 16 ? 4 * HR * DH : W * NA * ML * 16;
     static constexpr int SM = SM0 > 4096 ? SM0 : 4096;
@@ -103,9 +103,9 @@ __device__ __forceinline__ float quick_tanh(float z) {
 // scaled then, which took a fifth of a tile's vector instructions where every new maximum did.
 constexpr float LAZY = 8.0f;
 
-template <int DH, int BITS, int NHQ, bool WIN>
+template <int DH, int BITS, int NHQ, bool WIN, bool MANY = false>
 __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) {
-    using C = QuantCfg<DH, BITS, NHQ>;
+    using C = QuantCfg<DH, BITS, NHQ, MANY>;
     using Q = QuantRow<DH, BITS>;
     constexpr bool I4 = BITS == 4;
     constexpr int HR = C::HR, NA = C::NA, EV = C::EV, ROW = Q::ROW, G = Q::G, ML = C::ML, COLS = 2 * HR, W = C::W;
@@ -507,5 +507,13 @@ G4A_PAGED_QUANT_TYPES(64, 1, 4, 4) G4A_PAGED_QUANT_TYPES(64, 2, 4, 4) G4A_PAGED_
 G4A_PAGED_QUANT_TYPES(128, 1, 4, 4) G4A_PAGED_QUANT_TYPES(128, 2, 4, 4) G4A_PAGED_QUANT_TYPES(128, 4, 4, 4)
 G4A_PAGED_QUANT_TYPES(256, 1, 3, 3) G4A_PAGED_QUANT_TYPES(256, 2, 3, 3) G4A_PAGED_QUANT_TYPES(256, 4, 2, 2)
 G4A_PAGED_QUANT_TYPES(512, 1, 1, 1) G4A_PAGED_QUANT_TYPES(512, 2, 1, 1) G4A_PAGED_QUANT_TYPES(512, 4, 1, 1)
+// Many units of 512 dims: two workgroups of four waves a CU.
+#define G4A_PAGED_QUANT_MANY(type, bits, nhq)                                                                 \
+    extern "C" __global__ __launch_bounds__(256, 2) void g4a_paged_decode_many_d512_##type##_h##nhq(          \
+        G4aPagedAttnParams p) { paged_decode_quant<512, bits, nhq, false, true>(p); }                         \
+    extern "C" __global__ __launch_bounds__(256, 2) void g4a_paged_decode_many_win_d512_##type##_h##nhq(      \
+        G4aPagedAttnParams p) { paged_decode_quant<512, bits, nhq, true, true>(p); }
+G4A_PAGED_QUANT_MANY(i8, 8, 1) G4A_PAGED_QUANT_MANY(i8, 8, 2) G4A_PAGED_QUANT_MANY(i4, 4, 1) G4A_PAGED_QUANT_MANY(i4, 4, 2)
+#undef G4A_PAGED_QUANT_MANY
 #undef G4A_PAGED_QUANT_TYPES
 #undef G4A_PAGED_QUANT_DECODE

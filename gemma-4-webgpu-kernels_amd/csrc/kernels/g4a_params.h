@@ -443,5 +443,6 @@ struct G4aPagedAttnParams {
     float* part_ml;
 };
 
-// Waves of a workgroup of the decode over 8- and 4-bit pages, for 4 nhq query heads of dh dims.
-constexpr int g4a_paged_waves(int dh, int nhq) { return dh == 512 && nhq < 4 ? 8 : 4; }
+// Waves of a workgroup of the decode over 8- and 4-bit pages, for 4 nhq query heads of dh dims; `many`: units for every
+// CU, where two workgroups of four waves share one.
+constexpr int g4a_paged_waves(int dh, int nhq, bool many) { return dh == 512 && nhq < 4 && !many ? 8 : 4; }

@@ -352,7 +352,8 @@ def test_attention_long_and_ragged(ctx, kv_type):
 
 @pytest.mark.parametrize("n,hq,hkv,dh,kv_type,longest", [
     (2100, 2, 1, 64, "i4", 40), (1025, 8, 1, 64, "i8", 20), (300, 8, 8, 64, "i4", 40), (150, 40, 5, 128, "i8", 40),
-    (260, 8, 1, 512, "i4", 100), (140, 8, 1, 512, "i8", 100), (129, 4, 1, 512, "i4", 100), (65, 9, 1, 256, "i8", 300)])
+    (260, 8, 1, 512, "i4", 100), (140, 8, 1, 512, "i8", 100), (129, 4, 1, 512, "i4", 100), (65, 9, 1, 256, "i8", 300),
+    (150, 8, 2, 512, "i4", 60), (257, 7, 1, 512, "i8", 60), (256, 3, 1, 512, "i8", 60)])
 def test_attention_of_many_sequences(ctx, n, hq, hkv, dh, kv_type, longest):
     rng = np.random.default_rng(n)
     lens = rng.integers(0, longest + 1, n)

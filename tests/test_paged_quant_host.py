@@ -141,8 +141,16 @@ def test_launches(ctx, kv_type):  # noqa: F811
     assert names(ctx.kv_write_paged, c, PTR, PTR, PTR, 3) == [f"g4a_paged_write_d512_{kv_type}"]
     assert names(ctx.kv_read_paged, c, PTR, 3, PTR, PTR) == [f"g4a_paged_read_d512_{kv_type}"]
     assert names(ctx.kv_gather_paged, c, 1, 5, 100, PTR, PTR) == [f"g4a_paged_read_d512_{kv_type}"]
-    got = names(ctx.attention_paged, c, _attn())
-    assert len(got) == 2 and got[0].endswith(f"_d512_{kv_type}_h2") and got[1] == f"g4a_paged_combine16_d512_{kv_type}_h2"
+    got = names(ctx.attention_paged, _cache(kv_type=TYPES[kv_type], Dh=512, pages_per_seq=9), _attn())
+    assert got == [f"g4a_paged_decode_d512_{kv_type}_h2", f"g4a_paged_combine16_d512_{kv_type}_h2"]
+    # eight waves, a tile of 16 tokens each, are the smallest part there
+    assert names(ctx.attention_paged, c, _attn()) == got[:1]
+    # units for every CU: two workgroups of four waves a CU at 512 dims
+    many = _cache(kv_type=TYPES[kv_type], Dh=512, n_seqs=256)
+    assert names(ctx.attention_paged, many, _attn())[0] == f"g4a_paged_decode_many_d512_{kv_type}_h2"
+    assert names(ctx.attention_paged, many, _attn(Hq=3, sliding_window=90))[0] == f"g4a_paged_decode_many_win_d512_{kv_type}_h1"
+    assert names(ctx.attention_paged, many, _attn(Hq=9))[0] == f"g4a_paged_decode_d512_{kv_type}_h4"
+    assert names(ctx.attention_paged, _cache(kv_type=TYPES[kv_type], Dh=512, n_seqs=255), _attn())[0] == got[0]
     ctx.capture_begin()
     ctx.attention_paged(c, _attn())
     ctx.kv_write_paged(c, PTR, PTR, PTR, 3)
