@@ -107,6 +107,30 @@ __device__ __forceinline__ void paged_read(const G4aPagedRowsParams& p) {
         __builtin_nontemporal_store(x[e], reinterpret_cast<f32x4*>((VALUES ? p.v_out : p.k_out) + (size_t)row * DH + 4 * l + 256 * e));
 }
 
+// Sum of the LPR lanes (16, 32 or 64) that hold a row, in each of them: g4a_row_sum16 and the pairs, on two words.
+template <int CTRL>
+__device__ __forceinline__ double add_dpp64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false),
+                   hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+    return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int LPR>
+__device__ __forceinline__ double row_sum64(double x) {
+    x = add_dpp64<G4A_DPP_XOR1>(x);
+    x = add_dpp64<G4A_DPP_XOR2>(x);
+    x = add_dpp64<G4A_DPP_HALF_MIRROR>(x);
+    x = add_dpp64<G4A_DPP_ROW_MIRROR>(x);
+    auto pair = [](double y, auto swap) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, y);
+        const auto lo = swap((uint32_t)u), hi = swap((uint32_t)(u >> 32));
+        return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+    };
+    if constexpr (LPR >= 32) x = pair(x, [](uint32_t y) { return __builtin_amdgcn_permlane16_swap(y, y, false, false); });
+    if constexpr (LPR == 64) x = pair(x, [](uint32_t y) { return __builtin_amdgcn_permlane32_swap(y, y, false, false); });
+    return x;
+}
+
 // The K and V rows of the producer into pages of 8 and 4 bits: y = rope(x / sqrt(mean(x^2) + eps) * w) in 64 bits,
 // rounded once to f32 and then quantised. In f32, sums in another order (another width of the wave's work, another
 // device) would move a value over the border between two steps now and then, which 4 bits show: so the same rows
@@ -141,8 +165,7 @@ __device__ __forceinline__ void paged_produce_kv(const G4aPagedQuantProducerPara
             ss += y[4 * e + i] * y[4 * e + i];
         }
     }
-#pragma unroll
-    for (int d = 1; d < R::LPR; d *= 2) ss += __shfl_xor(ss, d);
+    ss = row_sum64<R::LPR>(ss);
     if (values || p.k_norm) {
         const double inv = 1.0 / sqrt(ss / DH + (double)p.eps);
 #pragma unroll
