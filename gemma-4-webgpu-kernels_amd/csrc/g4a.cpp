@@ -2366,7 +2366,11 @@ constexpr uint32_t PAGED_GRID = 0xFFFFFF;
 constexpr uint32_t PAGED_UNITS = 2048;
 // Its workgroups per CU (at 512 dims and up to 8 heads there is room for two, but most calls are faster with one:
 // 16 ragged sequences of f32 pages 40.4 us and 44.5, 256 of up to 1500 tokens 114 and 143, but 100 of up to 4000
-// 125 and 105):
+// 125 and 105. Pages of 8 and 4 bits, where a part's start and end weigh more beside its bytes, with the first number and with one more
+// a CU: 64 windows of 512 tokens of 256 dims in 4 bits 13.5 us and 14.6, 64 of up to 4000 in 8 bits 19.1 and 19.3, in 4 bits 18.2
+// and 17.4; 128 of up to 2000 of 4 groups of 4 heads of 128 dims 25.2 and 27.7; 64 of up to 4000 of 4 groups of 8 heads
+// with four 23.2, with three 24.9; 32 of 2 groups of 16 heads with two 15.1, with three 16.4; 64 dims with four
+// 19.4, with three 21.3):
 // [head_dim 64, 128, 256, 512][f32, bf16, 8-bit, 4-bit pages][4, 8, 16 heads a unit].
 constexpr uint32_t PAGED_WGS_PER_CU[4][4][3] = {
     {{4, 4, 2}, {4, 4, 4}, {4, 4, 4}, {4, 4, 4}},
@@ -2563,6 +2567,8 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
         return fail(ctx, G4A_E_SHAPE, "%u sequences of up to %u tokens in %u head groups: at most 2^31 tiles of 16 tokens",
                     cache->n_seqs, p.span, p.units);
     const bool quant = paged_quant(cache->kv_type);
+    // Units for every CU: 256 sequences of up to 1500 tokens in 4 bits 36.0 us with two workgroups of four waves a CU, 42.5 with one
+    // of eight; 128 of up to 4000, half as many units, 47.6 and 41.2.
     const bool many = quant && cache->Dh == 512 && h < 2 && uint64_t(cache->n_seqs) * p.units >= uint32_t(std::max(ctx->cu_count, 1));
     const uint32_t waves = quant ? g4a_paged_waves(int(cache->Dh), 1 << h, many) : 4;
     p.min_part = std::max(PAGED_MIN_PART, waves);
@@ -2573,7 +2579,9 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     // Parts to aim at where there are many units: at 512 dims and up to 8 heads half as many more, which the
     // second workgroup that a CU has room for takes (256 sequences of up to 1500 tokens, f32: 114 us with them,
     // 143 without, 127 with as many again; bf16 69, 82, 79; 100 of up to 4000, where there are fewer units, are not
-    // concerned).
+    // concerned). 8 and 4 bits: the same for the kernels of two workgroups a CU (256 of up to 1500 tokens in 4 bits 34.9 us,
+    // 38.4 without, 41.7 with as many again), and at 256 dims three times as many, where there is room for three
+    // (100 sequences of up to 300 tokens of 2 kv heads 12.5 us with them, 13.3 without).
     const uint32_t over = quant && d == 2 ? 3 * resident : (quant ? many : d == 3 && h < 2) ? resident + resident / 2 : resident;
     // launches of at most PAGED_UNITS units, which bounds the partials' memory, and of as many sequences as
     // the kernel counts

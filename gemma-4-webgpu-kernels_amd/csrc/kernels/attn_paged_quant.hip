@@ -1,6 +1,34 @@
-// Decode attention over pages of 8 and 4 bits for gfx950: as attn_paged.hip, whose
-// division of the work and merge these kernels share, on the whole numbers and
-// scales of paged_quant.h.
+// Decode attention over pages of 8 and 4 bits for gfx950: one query of every sequence over its visible tokens,
+//   out[b, h] = sum_t softmax_t(cap(scale * q[b, h] . K[t])) V[t],  K[t] = S_t sub n (8 bits: S_t n), V alike,
+// as attn_paged.hip, whose division of the work into parts and merge of their partials these kernels share. Formats:
+// paged_quant.h; layout: G4aPaged. The reference has no quantised cache.
+//
+// No value is ever multiplied out. sub n has 10 bits, so it is an fp16 operand exactly, made by one fma for two of them
+// (below); S_t, one number a token, goes to the score and to the probability:
+//   scores: K is the A operand of v_mfma_f32_16x16x32_f16 (lane = key l % 16 and a quarter of the dims, as it is loaded, no
+//           LDS in between), the query B, out of LDS, as two fp16 parts whose sum it is to 2^-22: 8 heads fill its 16
+//           columns. A lane then has four keys of one head; s = (x S) scale;
+//   softmax: in powers of two, relative to a maximum that follows the tiles' only when they pass it by LAZY, sum in f32;
+//   P.V:    P S_t 2^k is the A operand of v_mfma_f32_16x16x16_f16 as the softmax left it, in two fp16 parts in the rows of 8
+//           heads each, V is B: a lane holds four tokens' bytes of the same dims, and a byte permute pairs two
+//           tokens in a register. k follows the largest S_t, so that P S_t stays in fp16's range.
+// Against 64 bits the results are about as near as the same in f32 operations, or nearer (relative 5e-7 to 2e-6, those 6e-7
+// to 7e-6).
+//
+// A workgroup is 4 waves (8 at 512 dims, unless there are units for every CU), each on every 4th (8th) tile of its part
+// with the next tile's K and V in flight in registers, reloaded where they have been used. At 512 dims a wave holds 128
+// accumulators, so two waves a SIMD; eight waves that share their queries and one merge in LDS, and not two workgroups
+// of four: twice as many parts to start and merge (one sequence of 32768 tokens, 4 bits 17.6 us, 23.6 so; 16 ragged of up to 8192, 8 bits
+// 20.7 and 27.1). Where there are units for every CU the parts are there anyway, and two workgroups of four
+// overlap their starts and ends (256 sequences of up to 1500 tokens, 4 bits 36.0 us, 42.5 with eight waves).
+//
+// What bounds it: a tile of 512 dims and 8 heads in 4 bits takes about 450 vector instructions (some 150 each to unpack
+// K and V), 48 MFMAs and 8.8 KiB, and 590 instructions with its share of a wave's start and end: 2400 cycles of a SIMD, of the 3000 that
+// pass. So eight sequences of up to 131072 tokens (211 MB) take 49 us, 4.3 TB/s. Calls of few tiles a wave are bound by
+// the chain of a workgroup's start (lengths, table, queries: 5000 cycles; to the end of the first tile 10000), its end (6000) and
+// the merge launch (5 us).
+// A merge by the last of a unit's workgroups to end (tickets, partials past the XCD's cache) was slower:
+// 16 ragged sequences 26.5 us for 21, one window of 512 tokens 10.0 for 10.0.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

@@ -367,6 +367,8 @@ def test_attention_scale_softcap_and_page_stride(ctx, kv_type):
     _check(ctx, [100, 513, 31], 8, "scale", dh=256, scale=0.0625, unit=1.0, kv_type=kv_type, seed=1)
     _check(ctx, [100, 513, 31], 8, "a negative scale", dh=128, scale=-0.1, unit=1.0, kv_type=kv_type, seed=1)
     _check(ctx, [100, 513, 31], 8, "softcap", dh=512, cap=5.0, unit=1.0, kv_type=kv_type, seed=2)
+    for cap in (0.7, 40.0, 1000.0):  # scores far beyond the cap, about it and far below
+        _check(ctx, [100, 513, 31], 4, "softcap", dh=128, cap=cap, unit=1.0, kv_type=kv_type, seed=2)
     _check(ctx, [100, 513, 31], 8, "stride", dh=128, hkv=2, stride=quant.page_bytes(128, 2, 16, kv_type) + 48, kv_type=kv_type,
            seed=3)
 

@@ -82,6 +82,17 @@ def test_page_bytes(ctx, kv_type, dh, hkv, page):  # noqa: F811
     assert size(kv_type=0) == 4 * page * hkv * dh and size(kv_type=1, page_stride=page * hkv * dh + 8) == 2 * page * hkv * dh + 16
 
 
+def test_page_bytes_needs_no_context():
+    import ctypes
+    lib, n = hip.binding().load_library(), ctypes.c_uint64()
+    assert lib.g4a_kv_page_bytes(None, ctypes.byref(_cache(kv_type=4, Dh=512)), ctypes.byref(n)) == 0
+    assert n.value == quant.page_bytes(512, 1, 16, "i4")
+    assert lib.g4a_kv_page_bytes(None, ctypes.byref(_cache(kv_type=2)), ctypes.byref(n)) == ARG
+    assert b"kv_type" in lib.g4a_last_error(None)
+    assert lib.g4a_kv_page_bytes(None, None, ctypes.byref(n)) == ARG
+    assert lib.g4a_kv_page_bytes(None, ctypes.byref(_cache()), None) == ARG
+
+
 def test_page_bytes_refuses_and_leaves_a_capture_open(ctx):  # noqa: F811
     ctx.capture_begin()
     for code, text, kw in [(UNSUPPORTED, "page_size", dict(page_size=24)), (UNSUPPORTED, "head_dim", dict(Dh=96)),
