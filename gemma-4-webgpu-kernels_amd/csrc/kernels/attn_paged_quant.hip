@@ -242,8 +242,9 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
         if constexpr (PH >= 16) big = g4a_dpp_max<G4A_DPP_ROW_MIRROR>(big);
         if constexpr (PH >= 32) big = g4a_pair16_max(big);
         if constexpr (PH >= 64) big = g4a_pair32_max(big);
-        // times 2^(up - 127): the largest to [2^10, 2^11) (8 bits: [2^14, 2^15))
-        const uint32_t up = min(253u, 254u + (I4 ? 10u : 14u) - (big >> 23));
+        // times 2^(up - 127): the largest to [2^10, 2^11) (8 bits: [2^14, 2^15)), or by 2^122, of which 16 times is a
+        // number too: a query may be all zeros
+        const uint32_t up = min(249u, 254u + (I4 ? 10u : 14u) - (big >> 23));
         const float f = __uint_as_float(up << 23);
         if (ch == 0) k_s[h] = __uint_as_float((254u - up) << 23) * (I4 ? 0x1p6f : 0x1p3f);
         f16x8 hi, lo;

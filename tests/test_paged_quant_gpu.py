@@ -442,6 +442,20 @@ def test_attention_of_queries_that_are_not_finite(ctx, dh, hq, hkv, kv_type):
     c.free()
 
 
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("dh,hq", [(64, 16), (128, 3), (256, 8), (512, 9)])
+def test_attention_of_queries_of_nothing(ctx, kv_type, dh, hq):
+    """All zeros, the smallest numbers there are, and one value among zeros."""
+    c = Paged(ctx, [50, 700, 17, 33], dh=dh, kv_type=kv_type, seed=dh)
+    q = c.queries(hq)
+    q[0], q[1] = 0.0, q[1] * np.float32(1e-40)
+    q[2, :, 1:], q[3, 0] = 0.0, -0.0
+    got = c.attend(q)
+    want, bound = c.want(q)
+    _close(got, want, bound, "nothing")
+    c.free()
+
+
 def test_attention_is_repeatable_and_shares_pages(ctx):
     for kv_type in TYPES:
         c = Paged(ctx, [3000, 3000, 17], dh=512, page=32, kv_type=kv_type, seed=7)
