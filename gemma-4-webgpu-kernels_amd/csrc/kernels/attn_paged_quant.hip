@@ -269,7 +269,9 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     const float qf = k_s[key % HR] * p.scale * (p.softcap > 0.0f ? 1.0f : LOG2E);
     const float cap_inv = 1.0f / p.softcap;  // (where there is one)
     float m = G4A_NEG_INF, l = 0.0f;
-    float rs = 0x1p106f;  // P V's power of two: 2^6 over the largest S of V so far, rounded down to one
+    // P V's power of two: 2^6 over the largest S of V so far, rounded down to one (and as for 2^-100 for smaller S:
+    // the merge's factors, its reciprocal over a sum of up to 2^29, are not to be denormal)
+    float rs = 0x1p106f;
     f4v acc[NA];
 #pragma unroll
     for (int d = 0; d < NA; ++d) acc[d] = f4v{0.0f, 0.0f, 0.0f, 0.0f};

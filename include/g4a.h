@@ -623,7 +623,8 @@ int g4a_attn_producer_paged(g4a_ctx *ctx, const g4a_paged_cache *cache, const g4
  * several workgroups share stand in the context's workspace: run the call once, at
  * its sizes, before capturing it. Results are the same bits from call to call.
  * On pages of 8 and 4 bits queries and probabilities are held to 2^-22 of their value (or
- * 2^-35 of the largest of their head's, and 2^-31 of that of the tokens seen so far), sums in f32; a query row that
+ * 2^-35 of the largest of their head's, and 2^-31 of that of the tokens seen so far; query heads and V rows whose
+ * largest magnitude is below 2^-90 as if there were one that large), sums in f32; a query row that
  * holds an infinity or a NaN gives a row of NaN where it sees a token. */
 typedef struct g4a_paged_attn_args {
     const float *q; /* [n_seqs, Hq, Dh], 16-byte aligned */
