@@ -2574,6 +2574,10 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     p.min_part = std::max(PAGED_MIN_PART, waves);
     p.scale = a->scale;
     p.softcap = a->attn_softcap;
+    // Pages of 8 and 4 bits: the kernels multiply by 1 / cap and by cap * log2(e), which have to be finite. Under a
+    // cap of 2^126, as under any larger one, scores below 2^113 are themselves to f32's rounding, and larger ones so
+    // far apart that the largest takes all the weight; under caps up to 2^-126 every e^score is 1.
+    if (quant && p.softcap > 0.0f) p.softcap = std::min(std::max(p.softcap, 0x1p-126f), 0x1p126f);
     const int d = paged_dh(cache->Dh), t = paged_type(cache->kv_type);
     const uint32_t resident = uint32_t(std::max(ctx->cu_count, 1)) * PAGED_WGS_PER_CU[d][t][h];
     // Parts to aim at where there are many units: at 512 dims and up to 8 heads half as many more, which the

@@ -267,7 +267,7 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
     // lane (g4, n): keys 4 g4 + r of the tile, head n % HR of the unit; part n / HR % 2 of the queries and probabilities
     const bool lower = NHQ < 4 && key / HR % 2;
     const float qf = k_s[key % HR] * p.scale * (p.softcap > 0.0f ? 1.0f : LOG2E);
-    const float cap_inv = 1.0f / p.softcap;  // (where there is one)
+    const float cap_inv = 1.0f / p.softcap;  // (where there is one: from 2^-126 to 2^126)
     float m = G4A_NEG_INF, l = 0.0f;
     // P V's power of two: 2^6 over the largest S of V so far, rounded down to one (and as for 2^-100 for smaller S:
     // the merge's factors, its reciprocal over a sum of up to 2^29, are not to be denormal)

@@ -456,6 +456,21 @@ def test_attention_of_queries_of_nothing(ctx, kv_type, dh, hq):
     c.free()
 
 
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("dh,hq", [(64, 16), (128, 3), (256, 8), (512, 9)])
+def test_attention_of_soft_caps_at_the_ends_of_f32(ctx, kv_type, dh, hq):
+    """Caps beyond any score, up to f32's largest, leave scores as they are; caps down to its smallest make every score
+    about 0, one of exactly 0 among them."""
+    c = Paged(ctx, [100, 513, 31, 0, 7], dh=dh, kv_type=kv_type, seed=dh)
+    q = c.queries(hq)
+    q[2], q[4, 0] = 0.0, 0.0
+    for cap in (2.0 ** 126, 2.4e38, float(np.finfo(np.float32).max), 2.0 ** -126, 2e-39, 1e-45):
+        got = c.attend(q, cap=cap)
+        want, bound = c.want(q, cap=cap)
+        _close(got, want, bound, f"soft-cap {cap} dh {dh} {kv_type}")
+    c.free()
+
+
 def test_attention_is_repeatable_and_shares_pages(ctx):
     for kv_type in TYPES:
         c = Paged(ctx, [3000, 3000, 17], dh=512, page=32, kv_type=kv_type, seed=7)
