@@ -129,7 +129,7 @@ __device__ __forceinline__ float quick_tanh(float z) {
 }
 // Scores are relative to a maximum that follows the tiles' by more than this (of 2^x) alone: the accumulators are
 // scaled then, which took a fifth of a tile's vector instructions where every new maximum did.
-constexpr float LAZY = 8.0f;
+constexpr float LAZY = 8.0f, LEAST = 0x1p-8f;  // 2^-LAZY
 
 template <int DH, int BITS, int NHQ, bool WIN, bool MANY = false>
 __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) {
@@ -461,12 +461,15 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
         float f = mi == G4A_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
         // (a sum without a maximum: scores that are NaN)
         const float L = over_waves(mi == G4A_NEG_INF ? li : li * f, [](float a, float b) { return a + b; });
+        // (a partial's weights and their sum by 2^-LAZY: weights stand above 1 by up to 2^LAZY, where scores rise behind the
+        // maximum, and are not to take sums of V rows near f32's largest numbers past them)
         if (!whole && lane < HR) {
             float* const ml = p.part_ml + (size_t)at * 2 * HR + lane;
             ml[0] = M;
-            ml[HR] = L;
+            ml[HR] = L * LEAST;
         }
         if (whole) f *= L != 0.0f ? 1.0f / L : 0.0f;
+        else f *= LEAST;
         if (is) f_s[i][h] = f * r_s[i];
     }
     if constexpr (NHQ == 4) {

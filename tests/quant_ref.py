@@ -130,3 +130,31 @@ def attention(q, k, v, table, lens, *, scale=1.0, ring=False, **kw):
             score = 2.0 ** -22 * abs(scale) * np.linalg.norm(q[b, h]) * np.linalg.norm(kh, axis=1).max()
             wide[b, h] += (2 * score + 2.0 ** -22) * (p @ np.abs(vh)) + 2.0 ** -31 * len(kh) * np.abs(vh).max()
     return out, wide.reshape(bound.shape)
+
+
+def attention_sharp(q, k, v, table, lens, *, page, n_pages, ring=False, window=0, scale=1.0, cap=0.0):
+    """attention() for values of any magnitude and for long contexts: what fp16's last step costs a weight (2^-31 of the
+    largest value seen, and at least of 2^-90) is divided by the weights' sum, as the weight is, and nothing absolute is
+    added. The other terms are those of paged_ref.attention and attention()."""
+    n, hq, dh = q.shape
+    out, bound = np.zeros((n, hq, dh)), np.zeros((n, hq, dh))
+    opts = dict(page=page, ring=ring, n_pages=n_pages, window=window)
+    for b in range(n):
+        kk, vv = (ref.tokens(x, table, b, int(lens[b]), **opts)[1] for x in (k, v))
+        if not len(kk):
+            continue
+        for h in range(hq):
+            kh, vh = (x[:, h // (hq // k.shape[2])].astype(np.float64) for x in (kk, vv))
+            s = kh @ q[b, h].astype(np.float64)
+            length = np.linalg.norm(q[b, h]) * np.linalg.norm(kh, axis=1).max()
+            size = max(np.abs(s).max(), length / np.sqrt(dh))
+            s = s * scale
+            s = cap * np.tanh(s / cap) if cap else s
+            e = np.exp(s - s.max())
+            p = e / e.sum()
+            out[b, h] = p @ vh
+            steps = abs(scale) * size * (8 * np.sqrt(dh / 12) + 8) + 16 + 8 * np.sqrt(len(kh) / 12)
+            part = 2.0 ** -22 * (2 * abs(scale) * length + 1)
+            bound[b, h] = (2 * ref.HALF * steps + part) * (p @ np.abs(vh)) + 2.0 ** -31 * len(kh) / e.sum() * max(
+                np.abs(vh).max(), 2.0 ** -90)
+    return out.reshape(n, -1), bound.reshape(n, -1)

@@ -471,6 +471,53 @@ def test_attention_of_soft_caps_at_the_ends_of_f32(ctx, kv_type, dh, hq):
     c.free()
 
 
+def _values(c, b, x):
+    """Sequence b's V rows are x."""
+    t = np.arange(len(x))
+    c.put(1, c.table[b, t // c.page], t % c.page, x[:, None])
+
+
+def _sharp(c, q):
+    return quant.attention_sharp(q, *c.values(), c.table, c.lens, page=c.page, n_pages=c.n_pages)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("dh,hq", [(64, 16), (128, 3), (256, 8), (512, 9)])
+def test_attention_of_values_at_the_ends_of_f32(ctx, kv_type, dh, hq):
+    """V rows of 2^-110 or 2^-92 throughout, of 2^-110 ahead of 2^60 and behind it, and of 2^100, in parts that are their
+    whole unit and in those that are merged."""
+    c = Paged(ctx, [16, 60, 1100, 700, 900, 2000], dh=dh, kv_type=kv_type, seed=dh)
+    q = c.queries(hq)
+    for what, first, second in (("tiny", -110, -110), ("small", -92, -92), ("tiny, then large", -110, 60),
+                                ("large, then tiny", 60, -110), ("huge", 100, 100)):
+        for b, n in enumerate(c.lens):
+            power = np.where(np.arange(n) < n // 2, first, second)[:, None]
+            _values(c, b, c.rng.standard_normal((n, dh)) * 2.0 ** power)
+        c.upload()
+        _close(c.attend(q), *_sharp(c, q), f"{what} dh {dh} {kv_type}")
+    c.free()
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_attention_of_huge_values_under_rising_scores(ctx, kv_type):
+    """A maximum that lags behind the scores leaves weights above 1, by up to 2^8, and no sum of 32768 tokens' V rows of
+    2^108 passes f32's largest number for it. Two pages by turns: scores of 0, which a wave meets first, and of 5.4."""
+    dh, page, n = 256, 64, 32768
+    c = Paged(ctx, [2 * page], dh=dh, kv_type=kv_type, page=page, per_seq=n // page, seed=1)
+    low, high = c.table[0, :2]
+    c.table[0], c.lens[0] = np.tile([low, high], n // page // 2), n
+    c.put(0, np.full(page, low), np.arange(page), np.zeros((page, 1, dh)))
+    c.put(0, np.full(page, high), np.arange(page), np.full((page, 1, dh), 5.4))
+    for p in (low, high):
+        c.put(1, np.full(page, p), np.arange(page), c.rng.uniform(1, 2, (page, 1, dh)) * 2.0 ** 108)
+    c.upload()
+    ctx.h2d(c.dtable.ptr, c.table)
+    ctx.h2d(c.dlen.ptr, c.lens)
+    q = np.full((1, 2, dh), 1 / dh, np.float32)
+    _close(c.attend(q), *_sharp(c, q), f"rising scores {kv_type}")
+    c.free()
+
+
 def test_attention_is_repeatable_and_shares_pages(ctx):
     for kv_type in TYPES:
         c = Paged(ctx, [3000, 3000, 17], dh=512, page=32, kv_type=kv_type, seed=7)
