@@ -518,6 +518,33 @@ def test_attention_of_huge_values_under_rising_scores(ctx, kv_type):
     c.free()
 
 
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("dh,hq", [(64, 3), (256, 8), (512, 16)])
+def test_attention_holds_the_low_parts_of_probabilities_in_long_contexts(ctx, kv_type, dh, hq):
+    """9000 tokens whose weights, but for one of a tile's, lie between two fp16 numbers alike: without their low parts
+    the result would be off by some ten times its bound, as the host's form shows."""
+    n = 9000
+    c = Paged(ctx, [n], dh=dh, kv_type=kv_type, seed=dh)
+    t = np.arange(n)
+    k = np.zeros((n, 1, dh))
+    k[t % 16 == 0, 0, 0] = 127 / 128  # (a row of 8 bits has S = 2^-7, one of 4 bits S sub n = 1: scores of 0.677 are by q)
+    c.put(0, c.table[0, t // 16], t % 16, k)
+    v = c.rng.uniform(0.5, 1, (n, dh))
+    v[:, 1] = 1.0  # one S for all rows, 1.015625 times a power of two
+    _values(c, 0, v)
+    c.upload()
+    weight = (33 + 0.0146) / 65  # a weight times S and its power of two (to [64, 128)): a half step of fp16 off at 33
+    q = np.zeros((1, hq, dh), np.float32)
+    q[:, :, 0] = -np.log(weight) / c.values()[0][c.table[0, 0], 0, 0, 0]
+    want, bound = _sharp(c, q)
+    rows = c.values()[1][c.table[0, t // 16], t % 16, 0].astype(np.float64)
+    p = np.where(t % 16 == 0, 1.0, weight)
+    cut = (p * 65).astype(np.float16).astype(np.float64) @ rows / (65 * p.sum())
+    assert np.abs(cut - want[0, :dh]).min() > 5 * bound.max(), "a form that drops the low parts would pass"
+    _close(c.attend(q), want, bound, f"low parts dh {dh} {kv_type}")
+    c.free()
+
+
 def test_attention_is_repeatable_and_shares_pages(ctx):
     for kv_type in TYPES:
         c = Paged(ctx, [3000, 3000, 17], dh=512, page=32, kv_type=kv_type, seed=7)
