@@ -56,6 +56,35 @@ def test_the_format_against_fractions(kv_type):
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
+def test_how_far_a_value_may_be_off(kv_type):
+    """A half step against the largest magnitudes of row and group, as the binding's notes state it, in rows with and
+    without outliers. S is below its least real number by a factor of at most 1 + 2^-7 (bfloat16), 1016 / 1008 and 127 / 126;
+    |sub| is below its least real number + 1. So a step of 4 bits is below group / 8 + row / 1008."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((4000, 512)).astype(np.float32)
+    x[1000:] *= np.float32(2.0) ** rng.integers(-12, 3, (3000, 16)).repeat(32, axis=1).astype(np.float32)
+    x[np.arange(2000, 4000), rng.integers(0, 512, 2000)] = 10.0 ** rng.uniform(0, 4, 2000)
+    x[3000:] *= (2.0 ** rng.uniform(-116, 100, 1000)).astype(np.float32)[:, None]
+    off = np.abs(quant.values(x, kv_type).astype(np.float64) - x)
+    row = np.maximum(np.abs(x).max(-1), np.float32(2.0 ** -116 if kv_type == "i4" else 2.0 ** -119))[:, None].astype(np.float64)
+    if kv_type == "i8":
+        assert (off <= row / 252).all() and (off / row).max() > 0.98 / 252
+        return
+    g = x.reshape(4000, 16, 32).astype(np.float64)
+    group = np.abs(g).max(-1, keepdims=True)
+    half = (group / 16 + row[..., None] / 2016).repeat(32, -1)
+    opposite = np.where(g.max(-1, keepdims=True) >= -g.min(-1, keepdims=True), g < 0, g > 0)
+    off = off.reshape(g.shape)
+    assert (off < np.where(opposite, 2 * half, half)).all()
+    inner = np.where(opposite, 0, off / half)
+    assert inner.max() > 0.95 and (inner[2000:] > 1 / 16 * (group / half)[2000:]).any(), "not below 1/16 of the group's"
+    # a group far below its row's largest value
+    x = np.zeros(64, np.float32)
+    x[3], x[32:] = 1016.0, 0.45
+    assert not quant.values(x, kv_type)[32:].any() and quant.values(x, kv_type)[3] == 1016.0
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
 @pytest.mark.parametrize("vals", [False, True])
 @pytest.mark.parametrize("dh,hkv,page", [(64, 1, 16), (128, 3, 32), (256, 2, 16), (512, 1, 64)])
 def test_pages_hold_what_was_packed(kv_type, vals, dh, hkv, page):
