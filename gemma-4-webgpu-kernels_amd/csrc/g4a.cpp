@@ -2358,7 +2358,11 @@ constexpr uint32_t PAGED_SEQS = 1024;
 // Units up to which a merge block takes 16 items of one, not 64. (Sequences of up to 8192 tokens of 512 dims, a call
 // with 16 and with 64: 1 unit 32.3 us (32768 tokens) and 37.2, 2 18.7 and 21.3, 4 20.4 and 22.8, 8 26.5 and 27.7;
 // 12 34.7 and 36.0, 16 40.0 and 40.4, 24 56.8 and 55.6, 32 72.3 and 69.3. Windows of 512 tokens of 256 dims are within
-// 5 % either way up to 16 units, 32 16.5 and 16.4, 64 24.5 and 21.1.)
+// 5 % either way up to 16 units, 32 16.5 and 16.4, 64 24.5 and 21.1. Pages of 4 bits: 1 unit 16.9 and 21.1, 4 14.0 and
+// 15.5, 8 15.0 and 16.5, 12 16.9 and 17.6, 16 17.4 and 17.6, 24 22.6 and 21.0, 32 26.2 and 23.1; 8 bits alike; windows
+// 4 9.7 and 10.5, 16 10.6 and 11.2, 32 12.7 and 12.1, 64 17.4 and 13.3; 4 groups of 4 heads of 128 dims, 8 sequences of
+// up to 2000 tokens, 32 units, 9.9 and 11.1. So the border is a little low, by up to 0.7 us from 9 to 16 units, and by
+// more for that last form.)
 constexpr uint32_t PAGED_FEW_UNITS = 8;
 // Most workgroups of 256 threads of a launch: their threads along x are counted in 32 bits.
 constexpr uint32_t PAGED_GRID = 0xFFFFFF;
@@ -2366,11 +2370,11 @@ constexpr uint32_t PAGED_GRID = 0xFFFFFF;
 constexpr uint32_t PAGED_UNITS = 2048;
 // Its workgroups per CU (at 512 dims and up to 8 heads there is room for two, but most calls are faster with one:
 // 16 ragged sequences of f32 pages 40.4 us and 44.5, 256 of up to 1500 tokens 114 and 143, but 100 of up to 4000
-// 125 and 105. Pages of 8 and 4 bits, where a part's start and end weigh more beside its bytes, with the first number and with one more
-// a CU: 64 windows of 512 tokens of 256 dims in 4 bits 13.5 us and 14.6, 64 of up to 4000 in 8 bits 19.1 and 19.3, in 4 bits 18.2
-// and 17.4; 128 of up to 2000 of 4 groups of 4 heads of 128 dims 25.2 and 27.7; 64 of up to 4000 of 4 groups of 8 heads
-// with four 23.2, with three 24.9; 32 of 2 groups of 16 heads with two 15.1, with three 16.4; 64 dims with four
-// 19.4, with three 21.3):
+// 125 and 105. Pages of 8 and 4 bits, where a part's start and end weigh more beside its bytes, with the first number
+// and with one more a CU: 64 windows of 512 tokens of 256 dims in 4 bits 13.5 us and 14.6, 64 of up to 4000 in 8 bits
+// 19.1 and 19.3, but in 4 bits 18.2 and 17.4; 128 of up to 2000 of 4 groups of 4 heads of 128 dims 25.2 and 27.7; 64 of
+// up to 4000 of 4 groups of 8 heads with four 23.2, with three 24.9; 32 of 2 groups of 16 heads with two 15.1, with
+// three 16.4; 64 dims with four 19.4, with three 21.3):
 // [head_dim 64, 128, 256, 512][f32, bf16, 8-bit, 4-bit pages][4, 8, 16 heads a unit].
 constexpr uint32_t PAGED_WGS_PER_CU[4][4][3] = {
     {{4, 4, 2}, {4, 4, 4}, {4, 4, 4}, {4, 4, 4}},
@@ -2567,9 +2571,13 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
         return fail(ctx, G4A_E_SHAPE, "%u sequences of up to %u tokens in %u head groups: at most 2^31 tiles of 16 tokens",
                     cache->n_seqs, p.span, p.units);
     const bool quant = paged_quant(cache->kv_type);
-    // Units for every CU: 256 sequences of up to 1500 tokens in 4 bits 36.0 us with two workgroups of four waves a CU, 42.5 with one
-    // of eight; 128 of up to 4000, half as many units, 47.6 and 41.2.
-    const bool many = quant && cache->Dh == 512 && h < 2 && uint64_t(cache->n_seqs) * p.units >= uint32_t(std::max(ctx->cu_count, 1));
+    // Units for every CU: sequences in 4 bits with two workgroups of four waves a CU and with one of eight, 256 of up to
+    // 1500 tokens 35.3 us and 43.0 (8 bits 42.9 and 53.3), of up to 8000 94.4 and 118, of 300 23.9 and 28.4, windows of
+    // 512 28.3 and 34.5; 320 of up to 1500 48.5 and 48.8. Half as many units: 128 of up to 4000 47.6 and 41.2, of 1500
+    // 28.5 and 26.0. Between them the first is the faster one already (160 of up to 1500 29.1 and 35.3, 224 33.3 and
+    // 41.5; 192 of up to 4000 47.2 and 59.4), so this border could be lower.
+    const bool many = quant && cache->Dh == 512 && h < 2 &&
+                      uint64_t(cache->n_seqs) * p.units >= uint32_t(std::max(ctx->cu_count, 1));
     const uint32_t waves = quant ? g4a_paged_waves(int(cache->Dh), 1 << h, many) : 4;
     p.min_part = std::max(PAGED_MIN_PART, waves);
     p.scale = a->scale;
@@ -2583,10 +2591,13 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
     // Parts to aim at where there are many units: at 512 dims and up to 8 heads half as many more, which the
     // second workgroup that a CU has room for takes (256 sequences of up to 1500 tokens, f32: 114 us with them,
     // 143 without, 127 with as many again; bf16 69, 82, 79; 100 of up to 4000, where there are fewer units, are not
-    // concerned). 8 and 4 bits: the same for the kernels of two workgroups a CU (256 of up to 1500 tokens in 4 bits 34.9 us,
-    // 38.4 without, 41.7 with as many again), and at 256 dims three times as many, where there is room for three
-    // (100 sequences of up to 300 tokens of 2 kv heads 12.5 us with them, 13.3 without).
-    const uint32_t over = quant && d == 2 ? 3 * resident : (quant ? many : d == 3 && h < 2) ? resident + resident / 2 : resident;
+    // concerned). 8 and 4 bits: the same for the kernels of two workgroups a CU (256 of up to 1500 tokens in 4 bits 35.3
+    // us, 38.3 without, 42.5 with as many again, in 8 bits 42.9, 50.1, 49.9; of up to 4000 56.7, 68.0, 68.4; but 320 of up
+    // to 1500 48.7, 43.7, 47.2), and at 256 dims three times as many, where there is room for three (100 sequences of up
+    // to 300 tokens of 2 kv heads 12.4 us with them, 13.0 without).
+    const uint32_t over = quant && d == 2                           ? 3 * resident
+                          : (quant ? many : d == 3 && h < 2) ? resident + resident / 2
+                                                             : resident;
     // launches of at most PAGED_UNITS units, which bounds the partials' memory, and of as many sequences as
     // the kernel counts
     const uint32_t most = std::min({cache->n_seqs, std::max(1u, PAGED_UNITS / p.units), PAGED_SEQS});
@@ -2620,9 +2631,8 @@ int g4a_attention_paged(g4a_ctx* ctx, const g4a_paged_cache* cache, const g4a_pa
         p.out = all.out + size_t(b0) * a->Hq * cache->Dh;
         const uint32_t wgs = shares(p.c.n_seqs, &p.spread, &p.fit), units = p.c.n_seqs * p.units;
         const int win = a->sliding_window != 0;
-        if (int rc = launch(ctx, many ? ctx->paged_decode_many[win][t - 2][h] : ctx->paged_decode[win][d][t][h], dim3(wgs, 1, 1), dim3(64 * waves, 1, 1), p,
-                            "paged decode", true))
-            return rc;
+        const hipFunction_t decode = many ? ctx->paged_decode_many[win][t - 2][h] : ctx->paged_decode[win][d][t][h];
+        if (int rc = launch(ctx, decode, dim3(wgs, 1, 1), dim3(64 * waves, 1, 1), p, "paged decode", true)) return rc;
         if (!splits) continue;
         const uint32_t wide = units > PAGED_FEW_UNITS, blocks = uint32_t(item / 4) / (wide ? 64 : 16);
         if (int rc = launch(ctx, ctx->paged_combine[wide][d][t][h], dim3(blocks * units, 1, 1),

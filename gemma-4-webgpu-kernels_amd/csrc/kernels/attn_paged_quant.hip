@@ -20,11 +20,13 @@
 // accumulators, so two waves a SIMD; eight waves that share their queries and one merge in LDS, and not two workgroups
 // of four: twice as many parts to start and merge (one sequence of 32768 tokens, 4 bits 17.6 us, 23.6 so; 16 ragged of up to 8192, 8 bits
 // 20.7 and 27.1). Where there are units for every CU the parts are there anyway, and two workgroups of four
-// overlap their starts and ends (256 sequences of up to 1500 tokens, 4 bits 36.0 us, 42.5 with eight waves).
+// overlap their starts and ends (256 sequences of up to 1500 tokens, 4 bits 35.3 us, 43.0 with eight waves).
 //
 // What bounds it: a tile of 512 dims and 8 heads in 4 bits takes about 450 vector instructions (some 150 each to unpack
-// K and V), 48 MFMAs and 8.8 KiB, and 590 instructions with its share of a wave's start and end: 2400 cycles of a SIMD, of the 3000 that
-// pass. So eight sequences of up to 131072 tokens (211 MB) take 49 us, 4.3 TB/s. Calls of few tiles a wave are bound by
+// K and V), 48 MFMAs and 8.8 KiB, and 590 instructions with its share of a wave's start and end. Over eight sequences of
+// up to 131072 tokens (211 MB, 49 us with the merge, 4.3 TB/s) these are 2430 cycles of a SIMD a tile, two thirds of the
+// 3620 for which its waves live and half of the 4740 of the kernel: a quarter of it passes before a wave's start or after
+// its end, in the mean. Calls of few tiles a wave are bound by
 // the chain of a workgroup's start (lengths, table, queries: 5000 cycles; to the end of the first tile 10000), its end (6000) and
 // the merge launch (5 us).
 // A merge by the last of a unit's workgroups to end (tickets, partials past the XCD's cache) was slower:
@@ -521,11 +523,13 @@ __device__ __forceinline__ void paged_decode_quant(const G4aPagedAttnParams& p) 
 }  // namespace
 
 #define G4A_PAGED_QUANT_DECODE(dh, type, bits, nhq, occ)                                                      \
-    extern "C" __global__ __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), (occ * QuantCfg<dh, bits, nhq>::W / 4))                           \
+    extern "C" __global__                                                                                     \
+        __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), (occ * QuantCfg<dh, bits, nhq>::W / 4))          \
         void g4a_paged_decode_d##dh##_##type##_h##nhq(G4aPagedAttnParams p) {                                 \
         paged_decode_quant<dh, bits, nhq, false>(p);                                                          \
     }                                                                                                         \
-    extern "C" __global__ __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), (occ * QuantCfg<dh, bits, nhq>::W / 4))                           \
+    extern "C" __global__                                                                                     \
+        __launch_bounds__((64 * QuantCfg<dh, bits, nhq>::W), (occ * QuantCfg<dh, bits, nhq>::W / 4))          \
         void g4a_paged_decode_win_d##dh##_##type##_h##nhq(G4aPagedAttnParams p) {                             \
         paged_decode_quant<dh, bits, nhq, true>(p);                                                           \
     }                                                                                                         \

@@ -138,8 +138,10 @@ __device__ __forceinline__ double row_sum64(double x) {
 // rounded once to f32 and then quantised. In f32, sums in another order (another width of the wave's work, another
 // device) would move a value over the border between two steps now and then, which 4 bits show: so the same rows
 // give the same pages. The angle is position * frequency in f32, as for the query rows. The lanes hold a row as for
-// paged_write; a wave takes one group of K or of V rows of one token, and query rows waves of their own. 4099 tokens of 10 rows of
-// 256 (8 bits) take 21 us, 18.4 into f32 pages, whose K and V rows are in f32; 64 of 512 (4 bits) 5.3 and 3.7.
+// paged_write; a wave takes one group of K or of V rows of one token, and query rows waves of their own. 4099 tokens of
+// 10 rows of 256 (8 bits) take 21 us, 18.4 into f32 pages, whose K and V rows are in f32; 64 of 512 (4 bits) 5.3 and
+// 3.7: a chain of the position and slot, behind which the row is loaded (f32 pages load it beside them), its sum, root
+// and division in 64 bits, behind which the weights are, then frequencies and sines, then S and the subs.
 template <int DH, int BITS>
 __device__ __forceinline__ void paged_produce_kv(const G4aPagedQuantProducerParams& qp) {
     using R = RowLanes<DH>;
